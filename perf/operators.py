@@ -74,6 +74,7 @@ def draw(rng):
 def _quantise(x, most=127.0):
     """Rows of x in 8-bit integers and their scales, in the type of x."""
     a = x.abs().amax(dim=-1, keepdim=True)
+    most = torch.full_like(a, most)                # quotients of two tensors: a number's would be a product with its reciprocal
     inv = (most / a).clamp(max=FLT_MAX)
     fine = torch.isfinite(a)
     q = torch.where(fine, torch.round(x * inv), torch.zeros_like(x))
