@@ -340,6 +340,88 @@ int souffle_se_module_forward(const float* input, const float* w_reduce, const f
                               int32_t batch, int32_t channels, int32_t height, int32_t width, int32_t reduce, void* workspace,
                               size_t workspace_bytes, souffle_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------
+ * A residual block's norms, gate and residual scale in one pass (no counterpart in the reference):
+ *   u = N1(branch);  s = residual_scale * residual + branch_scale * gate * u;  o = N2(s)
+ * where N1 and N2 are each nothing, LayerNorm (weight and bias optional) or root-mean-square norm (weight optional):
+ *   layer: (x - mean) / sqrt(var + eps) * weight + bias;   rms: x / sqrt(mean(x^2) + eps) * weight.
+ * s and o are computed in fp32 from the unrounded values and rounded once, when they are stored.  With `out_q` the rows of o
+ * leave quantised as souffle_int8_quantize_rows would, from the unrounded values.
+ * Rows of a matrix are `*_stride` elements apart; strides of 16-byte multiples from 16-byte aligned addresses and a width
+ * that is a multiple of 8 take the vector path, anything else is read and written element by element.
+ * Asynchronous on `stream`; no workspace.
+ * ------------------------------------------------------------------------------------------ */
+enum { SOUFFLE_F32 = 0, SOUFFLE_F16 = 1, SOUFFLE_BF16 = 2 };
+enum { SOUFFLE_NORM_NONE = 0, SOUFFLE_NORM_LAYER = 1, SOUFFLE_NORM_RMS = 2 };
+typedef struct SouffleResidualNorm {
+  int32_t rows, cols;        /* rows >= 0, 1 <= cols <= 8192 */
+  int32_t dtype;             /* of residual, branch, sum, out: SOUFFLE_F32, _F16 or _BF16 */
+  int32_t param_dtype;       /* of gate, weights and biases: the same, or SOUFFLE_F32 */
+  int32_t branch_norm, out_norm;
+  int32_t gate_rows;         /* rows of `gate`; divides rows: rows / gate_rows consecutive rows share one.  0 without gate */
+  float residual_scale, branch_scale, branch_eps, out_eps;
+  int32_t reserved;          /* 0 */
+  int64_t residual_stride, branch_stride, sum_stride, out_stride, out_q_stride; /* elements */
+  const void* residual;      /* [rows][cols], or null: the residual term is left out */
+  const void* branch;        /* [rows][cols] */
+  const void* gate;          /* [gate_rows][cols], or null */
+  const void *branch_weight, *branch_bias, *out_weight, *out_bias; /* [cols], each may be null */
+  void* sum;                 /* [rows][cols], or null: s is not stored */
+  void* out;                 /* [rows][cols]; null without N2, and with out_q if only the quantised rows are wanted */
+  void* out_q;               /* int8 [rows][cols], or null */
+  float* out_scale;          /* [rows], with out_q */
+} SouffleResidualNorm;
+int souffle_residual_norm_forward(const SouffleResidualNorm* call, souffle_stream_t stream);
+
+/* The gradients of souffle_residual_norm_forward.  `f` describes the forward call; its sum, out, out_q and out_scale are not
+ * looked at: s is computed again from residual and branch, unrounded.  Null outputs are not computed; the gradients of a norm's
+ * weight and of a LayerNorm's bias exist whether or not the forward call had them (out_bias need not be given).  Gradients of
+ * vectors and gates are summed in fp32 in a fixed order (results do not change from run to run) and rounded once to
+ * param_dtype.  `workspace`: souffle_residual_norm_backward_workspace_bytes(rows, cols, gate_rows) bytes, 16-byte aligned, no state between calls. */
+typedef struct SouffleResidualNormGrad {
+  SouffleResidualNorm f;
+  int64_t grad_sum_stride, grad_out_stride, d_residual_stride, d_branch_stride; /* elements */
+  const void* grad_sum;      /* [rows][cols], or null (zero) */
+  const void* grad_out;      /* [rows][cols]; null without N2 */
+  void *d_residual, *d_branch;                                   /* [rows][cols] */
+  void* d_gate;                                                  /* [gate_rows][cols] */
+  void *d_branch_weight, *d_branch_bias, *d_out_weight, *d_out_bias; /* [cols] */
+  void* workspace;
+  size_t workspace_bytes;
+} SouffleResidualNormGrad;
+size_t souffle_residual_norm_backward_workspace_bytes(int32_t rows, int32_t cols, int32_t gate_rows);
+int souffle_residual_norm_backward(const SouffleResidualNormGrad* call, souffle_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Products in 8-bit integers with a scale per token and one per channel (no counterpart in the reference).
+ * Quantised rows: a = max |x| of the row, q = rint(x * min(127 / a, FLT_MAX)), half to even, scale = a / 127, all in fp32.  A row
+ * that holds an infinity or a NaN has scale NaN and q = 0; so its products are NaN.
+ * q's rows begin on 16-byte boundaries: base aligned, q_stride (bytes) a multiple of 16.
+ * ------------------------------------------------------------------------------------------ */
+int souffle_int8_quantize_rows(const void* x, int32_t dtype, int64_t x_stride, int32_t rows, int32_t cols, void* q, int64_t q_stride,
+                               float* scale, souffle_stream_t stream);
+/* out[m][n] = act(sum_k q[m][k] * w[n][k] * x_scale[m] * w_scale[n] + bias[n]); the sum is exact (32-bit integers), the rest
+ * fp32, rounded once.  x is int8 rows with x_scale, or floating rows, which are quantised on the way as above. */
+enum { SOUFFLE_I8 = 3 };
+enum { SOUFFLE_ACT_NONE = 0, SOUFFLE_ACT_RELU = 1, SOUFFLE_ACT_GELU = 2 /* tanh form */ };
+typedef struct SouffleInt8Linear {
+  int32_t rows, inner, cols; /* M >= 0, 1 <= K <= 131072 (the largest sum is then below 2^31), 1 <= N */
+  int32_t x_dtype;           /* SOUFFLE_F32, _F16, _BF16 or _I8 */
+  int32_t out_dtype;         /* of out and bias: SOUFFLE_F32, _F16 or _BF16 */
+  int32_t activation;
+  int64_t x_stride, w_stride, out_stride; /* elements; int8 rows begin on 16-byte boundaries */
+  const void* x;             /* [M][K] */
+  const float* x_scale;      /* [M] with int8 rows, otherwise null */
+  const void* w;             /* int8 [N][K] */
+  const float* w_scale;      /* [N] */
+  const void* bias;          /* [N], or null */
+  void* out;                 /* [M][N] */
+  void* workspace;           /* souffle_int8_linear_workspace_bytes(M, K, x_dtype), 16-byte aligned, no state between calls; null where that is 0 */
+  size_t workspace_bytes;
+} SouffleInt8Linear;
+size_t souffle_int8_linear_workspace_bytes(int32_t rows, int32_t inner, int32_t x_dtype);
+int souffle_int8_linear_forward(const SouffleInt8Linear* call, souffle_stream_t stream);
+
 /* Blocks until `stream` is idle, then decodes the status words in `workspace`. */
 int souffle_workspace_status(void* workspace, souffle_stream_t stream);
 /* Drops what the library remembers about a caller-owned workspace address (to be called before the memory is

@@ -12,6 +12,7 @@ import re
 import shutil
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -20,8 +21,10 @@ LIB_PATH = os.path.join(LIB_DIR, "libsouffle_b200.so")
 
 NVCC_FLAGS = [
     "-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
-    "-shared", "-Xcompiler", "-fPIC", "--cudart", "shared",
+    "-Xcompiler", "-fPIC", "--cudart", "shared",
 ]
+# the translation units: the megakernel, LSTM and squeeze-and-excite with their plans; the residual block's norms; 8-bit products
+UNITS = ("souffle_b200.cu", "residual_norm.cu", "int8_linear.cu")
 
 
 def _nvcc() -> str:
@@ -43,34 +46,38 @@ def is_stale() -> bool:
     return any(os.path.getmtime(s) > t for s in _sources())
 
 
+def _compile_all(out_dir: str, flags) -> str:
+    """Compiles every translation unit into `out_dir`, side by side; returns what nvcc printed."""
+    cmds = [[_nvcc(), *flags, "-c", "-o", os.path.join(out_dir, u[:-3] + ".o"), os.path.join(CSRC, u)] for u in UNITS]
+    runs = [subprocess.Popen(c, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True) for c in cmds]
+    said = [r.communicate()[0] for r in runs]
+    for r, text in zip(runs, said):
+        if r.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + text)
+    return "".join(said)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compiles csrc/souffle_b200.cu (which includes every kernel) into lib/libsouffle_b200.so."""
+    """Compiles the translation units and links them into lib/libsouffle_b200.so."""
     if not force and not is_stale():
         return LIB_PATH
     os.makedirs(LIB_DIR, exist_ok=True)
-    cmd = [_nvcc(), *NVCC_FLAGS, "-o", LIB_PATH, os.path.join(CSRC, "souffle_b200.cu")]
-    if verbose:
-        cmd.insert(1, "-Xptxas")
-        cmd.insert(2, "-v")
-    res = subprocess.run(cmd, capture_output=True, text=True)
+    with tempfile.TemporaryDirectory() as tmp:
+        said = _compile_all(tmp, [*NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else [])])
+        res = subprocess.run([_nvcc(), *NVCC_FLAGS, "-shared", "-o", LIB_PATH, *(os.path.join(tmp, u[:-3] + ".o") for u in UNITS)],
+                             capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
     if verbose:
-        sys.stderr.write(res.stderr)
+        sys.stderr.write(said)
     return LIB_PATH
 
 
 @functools.lru_cache(maxsize=None)
 def _ptxas_log() -> str:
-    """What `ptxas -v` prints for the library's one source file, compiled without linking."""
-    import tempfile
+    """What `ptxas -v` prints for the library's translation units, compiled without linking."""
     with tempfile.TemporaryDirectory() as tmp:
-        cmd = [_nvcc(), "-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-Xptxas", "-v", "-c",
-               "-o", os.path.join(tmp, "x.o"), os.path.join(CSRC, "souffle_b200.cu")]
-        res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
-    return res.stderr
+        return _compile_all(tmp, ["-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-Xptxas", "-v"])
 
 
 def stack_frames() -> dict:

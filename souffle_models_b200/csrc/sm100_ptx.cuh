@@ -32,7 +32,7 @@ __device__ __forceinline__ unsigned long long globaltimer_ns() {
   return t;
 }
 
-__device__ __noinline__ void record_timeout(const WaitCtl& c, int code, int where) {
+static __device__ __noinline__ void record_timeout(const WaitCtl& c, int code, int where) {
   *c.abort_smem = 1;
   if (atomicCAS(c.status_g, 0, code) == 0) {
     c.status_g[1] = where;
@@ -104,7 +104,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const W
 // The same for the lone lanes that feed the tensor core: the first tries stand in straight line and the loop is out of
 // line.  Behind a loop, a wait on a barrier that was complete already took 195 cycles, this form takes 60 (a try suspends
 // the thread for a while by itself before it fails, so few waits get as far as the loop).
-__device__ __noinline__ bool mbar_wait_loop(uint32_t bar, uint32_t parity, const WaitCtl& c, int where) {
+static __device__ __noinline__ bool mbar_wait_loop(uint32_t bar, uint32_t parity, const WaitCtl& c, int where) {
   return mbar_wait(bar, parity, c, where);
 }
 __device__ __forceinline__ bool mbar_wait_hot(uint32_t bar, uint32_t parity, const WaitCtl& c, int where) {

@@ -19,7 +19,7 @@
 #include <unordered_map>
 #include <vector>
 
-#include "../../include/souffle_b200.h"
+#include "host_common.h"
 #include "megakernel.cu"
 #include "lstm_kernel.cu"
 #include "lstm_static.cu"
@@ -28,11 +28,11 @@
 namespace souffle {
 
 // ------------------------------------------------------------------------------------
-// errors
+// errors, tensor maps (declared in host_common.h, shared with the other translation units)
 // ------------------------------------------------------------------------------------
 static thread_local std::string g_last_error;
 
-static int fail(int code, const char* fmt, ...) {
+int fail(int code, const char* fmt, ...) {
   char buf[512];
   va_list ap;
   va_start(ap, fmt);
@@ -41,23 +41,8 @@ static int fail(int code, const char* fmt, ...) {
   g_last_error = buf;
   return code;
 }
-#define SF_CUDA(call)                                                                          \
-  do {                                                                                         \
-    cudaError_t e_ = (call);                                                                   \
-    if (e_ != cudaSuccess)                                                                     \
-      return fail(SOUFFLE_CUDA_ERROR, "%s failed: %s (%s:%d)", #call, cudaGetErrorString(e_),  \
-                  __FILE__, __LINE__);                                                         \
-  } while (0)
 
-static bool aligned16(const void* p) { return p && (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-// ------------------------------------------------------------------------------------
-// tensor maps (driver entry point fetched at run time: no link-time libcuda dependency)
-// ------------------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static EncodeTiledFn encode_fn() {
+EncodeTiledFn encode_fn() {
   static EncodeTiledFn fn = nullptr;
   if (!fn) {
     void* p = nullptr;
@@ -67,6 +52,24 @@ static EncodeTiledFn encode_fn() {
       fn = reinterpret_cast<EncodeTiledFn>(p);
   }
   return fn;
+}
+
+int current_sms(int* sms_out, int* dev_out) {
+  static int known[kMaxDevices];                 // every thread that looks a device up finds the same number
+  int dev = 0;
+  SF_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= kMaxDevices) return fail(SOUFFLE_BAD_DEVICE, "device index %d out of range", dev);
+  if (!known[dev]) {
+    int major = 0, sms = 0;
+    SF_CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev));
+    SF_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    if (major != 10)
+      return fail(SOUFFLE_BAD_DEVICE, "device %d has compute capability %d.x; this library needs sm_100", dev, major);
+    known[dev] = sms;
+  }
+  *sms_out = known[dev];
+  if (dev_out) *dev_out = dev;
+  return SOUFFLE_OK;
 }
 
 // fp16 matrix [rows][cols] (cols contiguous), out-of-range elements read as zero; operand tiles are boxes of 64 columns x box_rows

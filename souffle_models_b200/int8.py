@@ -1,0 +1,112 @@
+"""Products in 8-bit integers with a scale per token and one per channel, over the C ABI (no counterpart in the reference):
+
+    out = activation(sum_k q[m, k] * w[n, k] * x_scale[m] * w_scale[n] + bias[n])
+
+`quantize_rows` makes the quantised rows of a matrix, `quantize_weight` those of a weight in the library's [K, N] layout,
+`int8_linear` is the product, of quantised rows or of floating ones that it quantises on the way, and `Int8Mlp` the MLP half of a BERT
+layer or Swin block on them.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from .residual_norm import residual_norm
+
+_ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2}
+
+
+def empty_rows(rows: int, cols: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Uninitialised (int8 [rows, cols], float32 [rows]) whose rows begin on 16-byte boundaries, as every quantised matrix's do."""
+    q = torch.empty(rows, (cols + 15) // 16 * 16, dtype=torch.int8, device=device)
+    return q[:, :cols], torch.empty(rows, dtype=torch.float32, device=device)
+
+
+def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(q int8 [rows, cols], scale float32 [rows]) of x [..., cols] (float32, float16, bfloat16): with a = max |x| of a row,
+    q = rint(x * min(127 / a, FLT_MAX)) and scale = a / 127; a row that holds an infinity or a NaN has scale NaN.  q's rows lie a
+    multiple of 16 bytes apart.  Asynchronous."""
+    code = _lib.DTYPE_CODES.get(x.dtype)
+    if not x.is_cuda or code is None:
+        raise ValueError("x must be a float32, float16 or bfloat16 CUDA tensor")
+    rows, cols, stride = _lib.rows_of(x, "x")
+    lib, stream = _lib.load(), _lib.stream_on(x.get_device())
+    q, scale = empty_rows(rows, cols, x.device)
+    _lib.check(lib.souffle_int8_quantize_rows(x.data_ptr(), code, stride, rows, cols, q.data_ptr(), (cols + 15) // 16 * 16, scale.data_ptr(), stream))
+    return q, scale
+
+
+def quantize_weight(w_kn: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """A weight [K, N], the layout of the library's fp16 products, as (int8 [N, K], float32 [N]) for int8_linear: a scale per
+    output channel.  To be done once."""
+    if w_kn.dim() != 2:
+        raise ValueError("weight must be [K, N]")
+    return quantize_rows(w_kn.t().contiguous())
+
+
+def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none",
+                x_scale: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """x [..., K], int8 with `x_scale` [rows] (see quantize_rows) or floating (quantised on the way); w int8 [N, K] with rows a multiple
+    of 16 bytes apart and w_scale [N] (see quantize_weight); bias [N] in the output's type; activation none, relu or gelu (tanh form).
+    Returns [..., N] in `out_dtype`, by default x's type, float16 for int8 rows.  K <= 131072.  Asynchronous."""
+    dev = x.get_device()
+    given = x.dtype == torch.int8
+    code = _lib.I8 if given else _lib.DTYPE_CODES.get(x.dtype)
+    if dev < 0 or code is None:
+        raise ValueError("x must be an int8, float32, float16 or bfloat16 CUDA tensor")
+    if out_dtype is None:
+        out_dtype = torch.float16 if given else x.dtype
+    out_code, act = _lib.DTYPE_CODES.get(out_dtype), _ACTIVATIONS.get(activation)
+    if out_code is None or act is None:
+        raise ValueError(f"out_dtype is float32, float16 or bfloat16 and activation {', '.join(_ACTIVATIONS)}: got {out_dtype}, {activation}")
+    rows, inner, stride = _lib.rows_of(x, "x", 16)
+    if w.dtype != torch.int8 or w.dim() != 2 or w.shape[1] != inner or w.get_device() != dev:
+        raise ValueError(f"w must be int8 [N, {inner}] on x's device")
+    cols, _, w_stride = _lib.rows_of(w, "w", 16)
+    if w_scale.dtype != torch.float32 or w_scale.shape != (cols,) or not w_scale.is_contiguous() or w_scale.get_device() != dev:
+        raise ValueError(f"w_scale must be a contiguous float32 tensor of {cols} values on x's device")
+    x_scale_ptr = bias_ptr = 0
+    if given != (x_scale is not None):
+        raise ValueError("x_scale comes with int8 rows and only with them")
+    if given:
+        if x_scale.dtype != torch.float32 or x_scale.numel() != rows or not x_scale.is_contiguous() or x_scale.get_device() != dev:
+            raise ValueError(f"x_scale must be a contiguous float32 tensor of {rows} values on x's device")
+        x_scale_ptr = x_scale.data_ptr()
+    if bias is not None:
+        if bias.dtype != out_dtype or bias.shape != (cols,) or not bias.is_contiguous() or bias.get_device() != dev:
+            raise ValueError(f"bias must be a contiguous {out_dtype} tensor of {cols} values on x's device")
+        bias_ptr = bias.data_ptr()
+    lib, stream = _lib.load(), _lib.stream_on(dev)
+    out = torch.empty(*x.shape[:-1], cols, dtype=out_dtype, device=x.device)
+    need = lib.souffle_int8_linear_workspace_bytes(rows, inner, code)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _lib.check(lib.souffle_int8_linear_forward(_lib.Int8Linear.pack(
+        rows, inner, cols, code, out_code, act, stride, w_stride, cols, x.data_ptr(), x_scale_ptr, w.data_ptr(), w_scale.data_ptr(), bias_ptr,
+        out.data_ptr(), ws.data_ptr() if need else 0, need), stream))
+    return out
+
+
+class Int8Mlp:
+    """The MLP half of an encoder layer on 8-bit products, from the fp16 weights that BertEncoder and SwinBlock take (fc1_w [C, F],
+    fc2_w [F, C], optional biases fc1_b, fc2_b and the norm's weight and bias):
+
+        norm_first=False (BERT):  LayerNorm(x + fc2(gelu(fc1(x))))        norm_first=True (Swin):  x + fc2(gelu(fc1(LayerNorm(x))))
+    """
+
+    def __init__(self, fc1_w: torch.Tensor, fc1_b: Optional[torch.Tensor], fc2_w: torch.Tensor, fc2_b: Optional[torch.Tensor],
+                 norm_g: Optional[torch.Tensor], norm_b: Optional[torch.Tensor], norm_first: bool = False, eps: float = 1e-5):
+        self.fc1, self.fc2 = quantize_weight(fc1_w), quantize_weight(fc2_w)
+        self.fc1_b, self.fc2_b, self.norm_g, self.norm_b = fc1_b, fc2_b, norm_g, norm_b
+        self.norm_first, self.eps = norm_first, eps
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        """x [..., C] of the biases' type -> the same shape and type; asynchronous."""
+        norm = dict(out_norm="layer", out_weight=self.norm_g, out_bias=self.norm_b, out_eps=self.eps, keep_sum=False)
+        if self.norm_first:          # the norm's rows leave in 8 bits: fc1 reads them as they are
+            q, scale = residual_norm(None, x, quantize=True, **norm)[1]
+            h = int8_linear(q, *self.fc1, bias=self.fc1_b, activation="gelu", x_scale=scale, out_dtype=x.dtype)
+            return residual_norm(x, int8_linear(h, *self.fc2, bias=self.fc2_b).view(x.shape))[0]
+        h = int8_linear(x, *self.fc1, bias=self.fc1_b, activation="gelu")
+        return residual_norm(x, int8_linear(h, *self.fc2, bias=self.fc2_b), **norm)[1]

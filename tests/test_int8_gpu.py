@@ -1,0 +1,238 @@
+"""Quantised rows and products in 8-bit integers against their definition.
+
+Quantised rows are compared bit for bit.  A product's sum is exact, so an output may be off by the roundings behind it: two products,
+the bias, at most 4 fp32 roundings (8 for GELU, whose slope is below 1.13, plus its exponential's few ulp) and the stored type's.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+FLOATS = [torch.float32, torch.float16, torch.bfloat16]
+FLT_MAX = torch.finfo(torch.float32).max
+
+
+def _int8():
+    from souffle_models_b200 import int8
+    return int8
+
+
+def _quantise(x):
+    x = x.float()
+    a = x.abs().amax(1, keepdim=True)
+    most = torch.full_like(a, 127.0)         # torch divides by a number as a product with its reciprocal, two tensors as it should
+    fine = torch.isfinite(a)
+    q = torch.where(fine, torch.round(x * (most / a).clamp(max=FLT_MAX)), torch.zeros_like(x))
+    return q.to(torch.int8), torch.where(fine, a / most, torch.full_like(a, math.nan)).reshape(-1)
+
+
+def _rows8(rows, cols, seed=0, most=127):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q, scale = _int8().empty_rows(rows, cols, "cuda")
+    q.copy_(torch.randint(-most, most + 1, (rows, cols), generator=g, device="cuda", dtype=torch.int8))
+    scale.copy_(torch.rand(rows, generator=g, device="cuda") * 0.02 + 0.001)
+    return q, scale
+
+
+def _product64(q, sx, w, sw, bias, act):
+    v = torch.cat([(a.double() @ w.double().t()) for a in q.split(2048)]) * sx.double()[:, None] * sw.double()
+    if bias is not None:
+        v = v + bias.double()
+    if act == "relu":
+        v = v.clamp(min=0)
+    elif act == "gelu":
+        v = 0.5 * v * (1 + torch.tanh(math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3)))
+    return v
+
+
+def _check(q, sx, w, sw, bias, act, out, x=None):
+    got = _int8().int8_linear(q if x is None else x, w, sw, bias=bias, activation=act, x_scale=sx if x is None else None, out_dtype=out)
+    want = _product64(q, sx, w, sw, bias, act)
+    linear = _product64(q, sx, w, sw, None, "none").abs() + (bias.double().abs() if bias is not None else 0)
+    bound = U[out] * want.abs() * 1.01 + 2.0 ** -24 * linear * (4 if act != "gelu" else 24)
+    if out == torch.float16:
+        bound = bound + 2.0 ** -25                          # half of the smallest fp16 step
+    err = (got.double() - want).abs()
+    assert got.dtype == out and bool((err <= bound).all()), (err.max().item(), (err / bound).max().item())
+    return got
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (5, 16), (4, 40), (2, 1000), (9, 1024), (3, 1025), (2, 4096), (3, 8200), (2, 20001), (1, 131072), (700, 768)])
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_quantised_rows_are_the_definitions(rows, cols, dtype):
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    x = (torch.randn(rows, cols, generator=g, device="cuda") * torch.exp(torch.randn(rows, 1, generator=g, device="cuda"))).to(dtype)
+    for m in (x, torch.cat([x, x], 1)[:, 3:3 + cols] if cols > 3 else x):
+        q, scale = _int8().quantize_rows(m)
+        want_q, want_scale = _quantise(m)
+        assert torch.equal(q, want_q) and torch.equal(scale, want_scale)
+        assert rows == 1 or q.stride(0) % 16 == 0
+
+
+def test_quantised_rows_of_zeros_infinities_and_the_ends_of_the_range():
+    x = torch.randn(9, 200, device="cuda")
+    x[0] = 0
+    x[1, 5] = math.inf
+    x[2, 199] = -math.inf
+    x[3, 0] = math.nan
+    x[4] *= 1e-43
+    x[5] *= 1e38 / x[5].abs().max()
+    x[6] = 127.0 * torch.arange(200, device="cuda") / 200.0 + 0.5
+    q, scale = _int8().quantize_rows(x)
+    want_q, want_scale = _quantise(x)
+    assert torch.equal(q, want_q) and torch.equal(scale.nan_to_num(-1), want_scale.nan_to_num(-1))
+    assert torch.isnan(scale).tolist() == [False, True, True, True] + [False] * 5
+    w, sw = _rows8(24, 200)
+    got = _int8().int8_linear(x, w, sw, activation="relu")
+    assert bool(torch.isnan(got[1:4]).all()) and bool((got[0] == 0).all()) and bool(torch.isfinite(got[[0, 4, 6, 7, 8]]).all())
+    # (row 5's products, near 1e38 * 127 * 0.01 * sqrt(200), lie beyond fp32's range)
+
+
+SIZES = [(1, 1, 1), (1, 768, 3072), (2, 16, 16), (3, 17, 5), (7, 3072, 768), (8, 64, 24), (9, 100, 33), (15, 1001, 130), (16, 48, 257), (17, 512, 64),
+         (31, 4096, 48), (33, 130, 1003), (64, 768, 768), (65, 16, 2048), (100, 1024, 96), (127, 300, 129), (128, 128, 128), (129, 65, 300), (196, 512, 2048),
+         (255, 2048, 512), (256, 96, 1000), (257, 768, 1024), (513, 1001, 515), (1000, 64, 64), (1571, 1001, 1003), (2048, 768, 2304), (2100, 777, 1030),
+         (4099, 128, 264), (300, 6000, 300)]
+
+
+@pytest.mark.parametrize("rows,inner,cols", SIZES)
+def test_products_of_quantised_rows(rows, inner, cols):
+    q, sx = _rows8(rows, inner, 1)
+    w, sw = _rows8(cols, inner, 2)
+    for k, out in enumerate(FLOATS):
+        bias = torch.randn(cols, device="cuda").to(out) if k != 1 else None
+        _check(q, sx, w, sw, bias, ("none", "gelu", "relu")[k], out)
+
+
+@pytest.mark.parametrize("rows,inner,cols", SIZES)
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_products_of_floating_rows(rows, inner, cols, dtype):
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = (torch.randn(rows, inner, generator=g, device="cuda") * torch.exp(0.5 * torch.randn(rows, 1, generator=g, device="cuda"))).to(dtype)
+    w, sw = _rows8(cols, inner, 2)
+    _check(*_quantise(x), w, sw, torch.randn(cols, device="cuda").to(dtype), "gelu", dtype, x=x)
+
+
+@pytest.mark.parametrize("rows,inner,cols", [(1, 131072, 3), (20, 131072, 17), (140, 131072, 130), (300, 131072, 300)])
+def test_sums_reach_the_end_of_32_bits(rows, inner, cols):
+    q, w = _int8().empty_rows(rows, inner, "cuda")[0].fill_(127), _int8().empty_rows(cols, inner, "cuda")[0].fill_(127)
+    w[::2] = -127
+    one = torch.ones(max(rows, cols), device="cuda")
+    got = _int8().int8_linear(q, w, one[:cols], x_scale=one[:rows], out_dtype=torch.float32)
+    want = torch.tensor(127 * 127 * inner, device="cuda").float() * torch.where(torch.arange(cols, device="cuda") % 2 == 0, -1.0, 1.0)
+    assert torch.equal(got, want.expand(rows, cols))
+
+
+@pytest.mark.parametrize("rows", [1, 16, 40, 300])
+def test_what_lies_between_the_rows_does_not_matter(rows):
+    inner, cols = 100, 70
+    q, sx = _rows8(rows, inner, 1)
+    w, sw = _rows8(cols, inner, 2)
+    want = _int8().int8_linear(q, w, sw, x_scale=sx)
+
+    def far(m, pitch):
+        room = torch.full((m.shape[0], pitch), 77, dtype=torch.int8, device="cuda")
+        room[:, :m.shape[1]] = m
+        return room[:, :m.shape[1]]
+
+    assert torch.equal(_int8().int8_linear(far(q, 112), far(w, 176), sw, x_scale=sx), want)
+    x = torch.randn(rows, inner + 9, device="cuda").half()
+    assert torch.equal(_int8().int8_linear(x[:, 3:3 + inner], w, sw), _int8().int8_linear(x[:, 3:3 + inner].contiguous(), w, sw))
+
+
+def test_offsets_beyond_32_bits():
+    rows, inner, cols, pitch = 40, 64, 16, 1 << 26
+    q, sx = _rows8(rows, inner, 1)
+    w, sw = _rows8(cols, inner, 2)
+    room = torch.empty(rows * pitch, dtype=torch.int8, device="cuda")         # the last rows lie beyond 2^31
+    far = room.view(rows, pitch)[:, :inner]
+    far.copy_(q)
+    assert torch.equal(_int8().int8_linear(far, w, sw, x_scale=sx), _int8().int8_linear(q, w, sw, x_scale=sx))
+    del far, room
+    big = 1 << 18                                                              # 2^18 x 10240 outputs: more than 2^31
+    q, sx = _rows8(big, 16, 1)
+    w, sw = _rows8(10240, 16, 2)
+    got = _int8().int8_linear(q, w, sw, x_scale=sx)
+    assert torch.equal(got[-300:], _int8().int8_linear(q[-300:], w, sw, x_scale=sx[-300:].contiguous()))
+
+
+def test_shapes_types_and_weights():
+    i8 = _int8()
+    w_kn = torch.randn(96, 40, device="cuda").half()
+    w, sw = i8.quantize_weight(w_kn)
+    want_w, want_sw = _quantise(w_kn.t())
+    assert torch.equal(w, want_w) and torch.equal(sw, want_sw)
+    x = torch.randn(2, 3, 96, device="cuda").half()
+    y = i8.int8_linear(x, w, sw)
+    assert y.shape == (2, 3, 40) and y.dtype == torch.float16
+    assert torch.equal(i8.int8_linear(x.view(6, 96), w, sw).view(2, 3, 40), y)
+    assert i8.int8_linear(x[0, 0], w, sw).shape == (40,)
+    assert i8.int8_linear(x[:0].reshape(0, 96), w, sw).shape == (0, 40)
+    # 8 bits cost a few per mille of the product's norm: two roundings of half a step out of 127 / 4 steps a deviation, over sqrt(3)
+    exact = x.double().view(6, 96) @ w_kn.double()
+    assert (y.double().view(6, 40) - exact).norm() < 0.03 * exact.norm()
+
+
+def test_refusals():
+    from souffle_models_b200 import SouffleError
+    i8 = _int8()
+    q, sx = _rows8(4, 64)
+    w, sw = _rows8(8, 64)
+    ok = dict(x=q, w=w, w_scale=sw, x_scale=sx)
+    i8.int8_linear(**ok)
+    for bad in (dict(x_scale=None), dict(x=q.half()), dict(w=w.half()), dict(w=w[:, :32]), dict(w_scale=sw.double()), dict(w_scale=sw[:4]), dict(x_scale=sx[:2]),
+                dict(activation="tanh"), dict(out_dtype=torch.float64), dict(bias=torch.zeros(8, device="cuda")), dict(x=q.cpu()), dict(x=q.to(torch.int32)),
+                dict(bias=torch.zeros(7, device="cuda").half())):
+        with pytest.raises(ValueError):
+            i8.int8_linear(**{**ok, **bad})
+    room = torch.zeros(4 * 72 + 64, dtype=torch.int8, device="cuda")
+    for bad in (dict(x=room[:4 * 72].view(4, 72)[:, :64]), dict(x=room[1:1 + 4 * 64].view(4, 64)), dict(x=q[:1].expand(4, 64))):
+        with pytest.raises(SouffleError):
+            i8.int8_linear(**{**ok, **bad})
+    long = torch.zeros(1, 131088, dtype=torch.int8, device="cuda")
+    with pytest.raises(SouffleError):
+        i8.int8_linear(long, long, sw[:1], x_scale=sx[:1])
+    for bad in (q, torch.zeros(4, 4), torch.zeros(4, 4, device="cuda").double(), torch.zeros(4, 6, device="cuda").t()):
+        with pytest.raises(ValueError):
+            i8.quantize_rows(bad)
+
+
+@pytest.mark.parametrize("rows", [5, 200])
+def test_on_another_stream_and_in_a_graph(rows):
+    i8 = _int8()
+    x = torch.randn(rows, 256, device="cuda").half()
+    w, sw = _rows8(96, 256)
+    want = i8.int8_linear(x, w, sw)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        i8.int8_linear(x, w, sw)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = i8.int8_linear(x, w, sw)
+    torch.cuda.current_stream().wait_stream(side)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("rows,norm_first", [(1, False), (1, True), (128, False), (196, True), (1000, False)])
+def test_mlp_half_of_a_layer(rows, norm_first):
+    """Against the same MLP on unquantised weights and activations: each of the two products is off by the two operands' roundings, half
+    a step out of about 127 / 4 steps a deviation, 1 / (2 sqrt(3)) of a step in the mean: 0.01 a product, and both norms keep that scale."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    make = lambda *s, std: (torch.randn(*s, generator=g, device="cuda") * std).half()
+    C, F = 512, 2048
+    p = dict(fc1_w=make(C, F, std=C ** -0.5), fc1_b=make(F, std=0.1), fc2_w=make(F, C, std=F ** -0.5), fc2_b=make(C, std=0.1),
+             norm_g=1 + make(C, std=0.1), norm_b=make(C, std=0.1))
+    x = make(rows, C, std=1.0)
+    y = _int8().Int8Mlp(**p, norm_first=norm_first).forward(x)
+    d = {k: v.double() for k, v in p.items()}
+    ln = lambda v: torch.nn.functional.layer_norm(v, (C,), d["norm_g"], d["norm_b"], 1e-5)
+    mlp = lambda v: torch.nn.functional.gelu(v @ d["fc1_w"] + d["fc1_b"], approximate="tanh") @ d["fc2_w"] + d["fc2_b"]
+    want = x.double() + mlp(ln(x.double())) if norm_first else ln(x.double() + mlp(x.double()))
+    assert y.shape == x.shape and y.dtype == torch.float16
+    assert (y.double() - want).norm() < 0.03 * want.norm()

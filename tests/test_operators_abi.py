@@ -1,0 +1,118 @@
+"""Call records of the residual block's operators: layout, and refusals that need no device."""
+import ctypes as C
+import os
+import subprocess
+
+import pytest
+import torch
+
+from souffle_models_b200 import _lib, int8, residual_norm
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def test_call_records_have_the_headers_layout(tmp_path):
+    records = {"SouffleResidualNorm": _lib.ResidualNorm, "SouffleResidualNormGrad": _lib.ResidualNormGrad, "SouffleInt8Linear": _lib.Int8Linear}
+    src = '#include <stdio.h>\n#include <stddef.h>\n#include "souffle_b200.h"\nint main(void) {\n'
+    for name, r in records.items():
+        src += f'  printf("{name} %zu\\n", sizeof({name}));\n'
+        for f, _ in r.structure._fields_:
+            at = "f." + f if name == "SouffleResidualNormGrad" and f in dict(_lib.ResidualNorm.structure._fields_) else f
+            src += f'  printf("{name}.{f} %zu\\n", offsetof({name}, {at}));\n'
+    (tmp_path / "t.c").write_text(src + "  return 0;\n}\n")
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), "-o", str(tmp_path / "t"), str(tmp_path / "t.c")], check=True)
+    out = dict(line.rsplit(" ", 1) for line in subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, check=True).stdout.splitlines())
+    for name, r in records.items():
+        assert int(out[name]) == C.sizeof(r.structure) == len(r.pack(*([0] * len(r.structure._fields_))))
+        for f, _ in r.structure._fields_:
+            assert int(out[f"{name}.{f}"]) == getattr(r.structure, f).offset, f
+
+
+def _norm(**kw):
+    d = _lib.ResidualNorm.structure(rows=4, cols=64, dtype=1, param_dtype=1, out_norm=1, residual_scale=1, branch_scale=1, branch_eps=1e-5, out_eps=1e-5,
+                                    residual_stride=64, branch_stride=64, sum_stride=64, out_stride=64, residual=4096, branch=8192, sum=12288, out=16384)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(rows=-1), 1), (dict(cols=0), 1), (dict(cols=8193, residual_stride=8193), 1), (dict(dtype=3), 7), (dict(param_dtype=2), 7), (dict(branch_norm=3), 7),
+    (dict(out_eps=-1.0), 7), (dict(branch_eps=float("nan")), 7), (dict(branch_weight=4096), 7), (dict(out_norm=2, out_bias=4096), 7), (dict(gate_rows=2), 1),
+    (dict(gate=4096), 1), (dict(gate=4096, gate_rows=3), 1), (dict(branch=None), 2), (dict(branch_stride=63), 1), (dict(sum_stride=63), 1),
+    (dict(out_norm=0), 7), (dict(out=None, sum=None), 2), (dict(out_q=4096), 1), (dict(out_q=4096, out_q_stride=64), 2),
+    (dict(out_q=4104, out_q_stride=64, out_scale=4096), 2), (dict(out_q=4096, out_q_stride=72, out_scale=4096), 2), (dict(branch=8193), 2), (dict(out_weight=4097), 2),
+])
+def test_norms_refuse(change, code):
+    lib = _lib.load()
+    d = _norm(**change)
+    assert lib.souffle_residual_norm_forward(C.addressof(d), None) == code, lib.souffle_last_error()
+    assert lib.souffle_last_error()
+
+
+def test_null_records_and_empty_calls():
+    lib = _lib.load()
+    for fn in (lib.souffle_residual_norm_forward, lib.souffle_residual_norm_backward, lib.souffle_int8_linear_forward):
+        assert fn(None, None) == 7
+    d = _norm(rows=0)
+    assert lib.souffle_residual_norm_forward(C.addressof(d), None) == 0
+    assert lib.souffle_int8_quantize_rows(None, 1, 64, 0, 64, None, 64, None, None) == 0
+
+
+@pytest.mark.parametrize("change,code", [(dict(), 2), (dict(grad_out=4096), 1), (dict(grad_out=4096, grad_out_stride=64), 2),
+                                         (dict(grad_out=4096, grad_out_stride=64, d_gate=4096), 7), (dict(grad_out=4096, grad_out_stride=64, d_branch_bias=4096), 7),
+                                         (dict(out_norm=0, out=None), 2)])
+def test_gradients_refuse(change, code):
+    lib = _lib.load()
+    d = _lib.ResidualNormGrad.structure()
+    front = _norm()
+    C.memmove(C.addressof(d), C.addressof(front), C.sizeof(_lib.ResidualNorm.structure))
+    for k, v in change.items():
+        setattr(d, k, v)
+    assert lib.souffle_residual_norm_backward(C.addressof(d), None) == code, lib.souffle_last_error()
+
+
+def test_workspaces_hold_what_the_kernels_write():
+    lib = _lib.load()
+    assert lib.souffle_residual_norm_backward_workspace_bytes(0, 64, 0) == 0
+    assert lib.souffle_residual_norm_backward_workspace_bytes(1, 64, 0) >= 5 * 64 * 4
+    assert lib.souffle_residual_norm_backward_workspace_bytes(10 ** 6, 8192, 4) > lib.souffle_residual_norm_backward_workspace_bytes(10 ** 6, 8192, 1) > 0
+    assert lib.souffle_int8_linear_workspace_bytes(5, 100, _lib.I8) == 0
+    assert lib.souffle_int8_linear_workspace_bytes(5, 100, 1) >= 5 * 112 + 5 * 4
+    assert lib.souffle_int8_linear_workspace_bytes(1 << 20, 1 << 17, 1) > 1 << 37       # no 32-bit product on the way
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(rows=-1), 1), (dict(inner=0), 1), (dict(inner=131073, x_stride=131088, w_stride=131088), 1), (dict(cols=0), 1), (dict(x_dtype=4), 7), (dict(out_dtype=3), 7),
+    (dict(activation=3), 7), (dict(x_stride=48), 1), (dict(x_stride=72), 1), (dict(w_stride=72), 1), (dict(out_stride=7), 1), (dict(x_scale=None), 7),
+    (dict(x_dtype=1), 7), (dict(x=None), 2), (dict(x=4104), 2), (dict(w=4104), 2), (dict(w_scale=None), 2), (dict(bias=4097), 2), (dict(out=None), 2),
+    (dict(x_dtype=1, x_scale=None), 2), (dict(x_dtype=1, x_scale=None, workspace=4096, workspace_bytes=16), 2),
+])
+def test_products_refuse(change, code):
+    lib = _lib.load()
+    d = _lib.Int8Linear.structure(rows=4, inner=64, cols=8, x_dtype=_lib.I8, out_dtype=1, x_stride=64, w_stride=64, out_stride=8, x=4096, x_scale=4096, w=4096,
+                                  w_scale=4096, out=4096)
+    for k, v in change.items():
+        setattr(d, k, v)
+    assert lib.souffle_int8_linear_forward(C.addressof(d), None) == code, lib.souffle_last_error()
+
+
+def test_rows_of_tensors():
+    rows_of = _lib.rows_of
+    x = torch.zeros(6, 20)
+    assert rows_of(x, "x") == (6, 20, 20) and rows_of(x[:, :7], "x") == (6, 7, 20) and rows_of(x.view(2, 3, 20), "x") == (6, 20, 20)
+    assert rows_of(x[:1, :7], "x") == (1, 7, 8) and rows_of(x[0, :7], "x", 16) == (1, 7, 16) and rows_of(x[::2], "x") == (3, 20, 40)
+    assert rows_of(x[:0], "x")[0] == 0
+    for bad in (x.t(), x.view(2, 3, 20)[:, :, :7], torch.zeros(())):
+        with pytest.raises(ValueError):
+            rows_of(bad, "x")
+
+
+def test_tensors_on_the_cpu_are_refused():
+    x = torch.zeros(4, 64)
+    with pytest.raises(ValueError):
+        residual_norm.residual_norm(x, x)
+    with pytest.raises(ValueError):
+        int8.quantize_rows(x)
+    with pytest.raises(ValueError):
+        int8.int8_linear(x, torch.zeros(8, 64, dtype=torch.int8), torch.zeros(8))

@@ -1,0 +1,330 @@
+"""Norms, gate and residual scale around a block, forward and backward, against the formulas in 64 bits.
+
+Tolerances.  U is the unit roundoff of the stored type.  A stored value may be off by U |value|; on top come the fp32 operations behind
+it: a row's sums are chains of at most 8 * 4 additions in a thread, 5 over a warp, 8 over warps, so a mean is off by less than
+64 * 2^-24 of the row's largest magnitude, and what is built from it by a small multiple (kSlack).  Sums over rows are chains of at most
+`rows` + 64 additions of terms that carry such an error themselves.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+E32 = 2.0 ** -24
+KINDS = [("none", "layer"), ("none", "rms"), ("layer", "layer"), ("rms", "rms"), ("layer", "none"), ("rms", "layer"), ("none", "none")]
+TYPES = [(torch.float32, torch.float32), (torch.float16, torch.float16), (torch.float16, torch.float32), (torch.bfloat16, torch.bfloat16),
+         (torch.bfloat16, torch.float32)]
+
+
+def _rn():
+    from souffle_models_b200 import residual_norm
+    return residual_norm
+
+
+def _make(rows, cols, dtype, params, n1, n2, gates, seed=0, residual=True):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    randn = lambda *s, std=1.0: torch.randn(*s, generator=g, device="cuda") * std
+    t = dict(residual=(randn(rows, cols, std=2.0).to(dtype) if residual else None), branch=(randn(rows, cols) + 0.3).to(dtype),
+             gate=(0.5 + randn(gates, cols, std=0.2)).to(params) if gates else None)
+    for k, n in (("branch", n1), ("out", n2)):
+        t[k + "_weight"] = (1 + randn(cols, std=0.1)).to(params) if n != "none" else None
+        t[k + "_bias"] = randn(cols, std=0.1).to(params) if n == "layer" else None
+    return t
+
+
+def _norm64(x, kind, w, b, eps):
+    if kind == "none":
+        return x
+    m = x.mean(1, keepdim=True) if kind == "layer" else torch.zeros_like(x[:, :1])
+    x = (x - m) / torch.sqrt(((x - m) ** 2).mean(1, keepdim=True) + eps)
+    if w is not None:
+        x = x * w
+    return x if b is None else x + b
+
+
+def _formula(t, n1, n2, alpha, beta, eps=1e-5):
+    """(s, o) in 64 bits."""
+    d = {k: None if v is None else v.double() if v.dtype != torch.float64 else v for k, v in t.items()}
+    u = _norm64(d["branch"], n1, d["branch_weight"], d["branch_bias"], eps)
+    if d["gate"] is not None:
+        u = u * d["gate"].repeat_interleave(u.shape[0] // d["gate"].shape[0], 0)
+    s = beta * u + (alpha * d["residual"] if d["residual"] is not None else 0)
+    return s, _norm64(s, n2, d["out_weight"], d["out_bias"], eps) if n2 != "none" else None
+
+
+def _near(got, want, slack, what):
+    """|got - want| within U |want| + slack (a tensor or number), element by element."""
+    err = (got.double() - want).abs()
+    bound = U[got.dtype] * want.abs() * 1.01 + slack
+    assert bool((err <= bound).all()), (what, err.max().item(), (err / bound).max().item())
+
+
+def _row_slack(t, n1, n2, alpha, beta, eps=1e-5):
+    """What fp32 may cost s and o, row by row (column vectors)."""
+    d = {k: None if v is None else v.double() for k, v in t.items()}
+    most = lambda x: 0.0 if x is None else x.abs().amax().item()
+    y = d["branch"].abs().amax(1, keepdim=True)
+    if n1 != "none":
+        y = d["branch"]
+        dev = torch.sqrt((y.var(1, unbiased=False, keepdim=True) if n1 == "layer" else (y * y).mean(1, keepdim=True)) + eps)
+        y = y.abs().amax(1, keepdim=True) / dev * (most(d["branch_weight"]) or 1.0) + most(d["branch_bias"])
+    es = 64 * E32 * (abs(beta) * y * (most(d["gate"]) or 1.0) + (abs(alpha) * d["residual"].abs().amax(1, keepdim=True) if d["residual"] is not None else 0))
+    if n2 == "none":
+        return es, None
+    s = _formula(t, n1, n2, alpha, beta, eps)[0]
+    dev = torch.sqrt((s.var(1, unbiased=False, keepdim=True) if n2 == "layer" else (s * s).mean(1, keepdim=True)) + eps)
+    top = s.abs().amax(1, keepdim=True)
+    eo = (2 * es * (1 + (top / dev)) / dev + 64 * E32 * top / dev * (1 + top / dev)) * (most(d["out_weight"]) or 1.0) + 4 * E32 * most(d["out_bias"])
+    return es, eo
+
+
+SHAPES = [(1, 1), (2, 7), (3, 33), (5, 64), (17, 255), (4, 256), (6, 264), (33, 513), (31, 768), (9, 1001), (7, 1024), (5, 1032), (3, 2049), (6, 4096),
+          (3, 4104), (2, 8191), (3, 8192)]
+
+
+@pytest.mark.parametrize("rows,cols", SHAPES)
+@pytest.mark.parametrize("n1,n2", KINDS)
+def test_forward_at_odd_and_even_widths(rows, cols, n1, n2):
+    for k, (dtype, params) in enumerate(TYPES[::2]):
+        t = _make(rows, cols, dtype, params, n1, n2, gates=(0, 1, rows)[k], seed=k)
+        s, o = _rn().residual_norm(t["residual"], t["branch"], branch_norm=n1, branch_weight=t["branch_weight"], branch_bias=t["branch_bias"],
+                                   gate=t["gate"], out_norm=n2, out_weight=t["out_weight"], out_bias=t["out_bias"], residual_scale=0.9,
+                                   branch_scale=1.25)
+        want_s, want_o = _formula(t, n1, n2, 0.9, 1.25)
+        es, eo = _row_slack(t, n1, n2, 0.9, 1.25)
+        _near(s, want_s, es, "s")
+        if n2 == "none":
+            assert o is None
+        else:
+            _near(o, want_o, eo, "o")
+
+
+@pytest.mark.parametrize("dtype,params", TYPES)
+@pytest.mark.parametrize("gates", [0, 1, 3, 12])
+def test_forward_types_gates_and_missing_parts(dtype, params, gates):
+    t = _make(12, 776, dtype, params, "layer", "layer", gates)
+    want_s, want_o = _formula(t, "layer", "layer", 1.0, 1.0)
+    es, eo = _row_slack(t, "layer", "layer", 1.0, 1.0)
+    kw = dict(branch_norm="layer", branch_weight=t["branch_weight"], branch_bias=t["branch_bias"], gate=t["gate"], out_norm="layer",
+              out_weight=t["out_weight"], out_bias=t["out_bias"])
+    s, o = _rn().residual_norm(t["residual"], t["branch"], **kw)
+    _near(s, want_s, es, "s")
+    _near(o, want_o, eo, "o")
+    none, alone = _rn().residual_norm(t["residual"], t["branch"], keep_sum=False, **kw)
+    assert none is None and torch.equal(alone, o)
+    shaped = _rn().residual_norm(t["residual"].view(3, 4, 776), t["branch"].view(3, 4, 776), **kw)
+    assert torch.equal(shaped[0].view(12, 776), s) and torch.equal(shaped[1].view(12, 776), o)
+    t.update(residual=None, branch_weight=None, out_bias=None)
+    kw.update(branch_weight=None, out_bias=None)
+    s, o = _rn().residual_norm(None, t["branch"], **kw)
+    want_s, want_o = _formula(t, "layer", "layer", 1.0, 1.0)
+    es, eo = _row_slack(t, "layer", "layer", 1.0, 1.0)
+    _near(s, want_s, es, "s without residual")
+    _near(o, want_o, eo, "o without residual")
+
+
+def test_rows_that_lie_apart_and_addresses_that_are_not_aligned():
+    rows, cols = 9, 264
+    for off, pitch in ((0, 272), (1, 271), (8, 264 + 3)):
+        t = _make(rows, cols, torch.float16, torch.float32, "rms", "layer", 3)
+        far = lambda x: torch.zeros(rows * pitch + off, dtype=x.dtype, device="cuda")[off:].view(rows, pitch)[:, :cols].copy_(x)
+        kw = dict(branch_norm="rms", branch_weight=t["branch_weight"], gate=t["gate"], out_norm="layer", out_weight=t["out_weight"],
+                  out_bias=t["out_bias"])
+        s, o = _rn().residual_norm(t["residual"], t["branch"], **kw)
+        want_s, want_o = _formula(t, "rms", "layer", 1.0, 1.0)
+        es, eo = _row_slack(t, "rms", "layer", 1.0, 1.0)
+        s2, o2 = _rn().residual_norm(far(t["residual"]), far(t["branch"]), **kw)
+        for got_s, got_o in ((s, o), (s2, o2)):
+            _near(got_s, want_s, es, "s")
+            _near(got_o, want_o, eo, "o")
+        ds, do = torch.randn_like(t["branch"]), torch.randn_like(t["branch"])
+        kw.pop("out_bias")
+        a = _rn().residual_norm_backward(ds, do, t["residual"], t["branch"], **kw)
+        b = _rn().residual_norm_backward(far(ds), far(do), far(t["residual"]), far(t["branch"]), **kw)
+        for k in a:
+            if a[k] is not None:
+                assert (a[k].double() - b[k].double()).norm() <= 2 * U[a[k].dtype] * a[k].double().norm() + 1e-5 * a[k].double().norm(), k
+
+
+def test_offsets_beyond_32_bits():
+    rows, cols, pitch = 3, 64, (1 << 30) + 8
+    t = _make(rows, cols, torch.float16, torch.float16, "none", "layer", 0)
+    room = torch.empty(2 * pitch + cols, dtype=torch.float16, device="cuda")
+    far = room.as_strided((rows, cols), (pitch, 1))
+    far.copy_(t["branch"])
+    kw = dict(out_norm="layer", out_weight=t["out_weight"], out_bias=t["out_bias"])
+    assert torch.equal(_rn().residual_norm(t["residual"], far, **kw)[1], _rn().residual_norm(t["residual"], t["branch"], **kw)[1])
+
+
+def test_rows_of_zeros_infinities_and_no_rows():
+    t = _make(8, 768, torch.float16, torch.float16, "none", "layer", 0)
+    t["residual"][1:3] = 0
+    t["branch"][1:3] = 0
+    t["branch"][5, 17] = float("inf")
+    t["branch"][6, 3] = float("nan")
+    kw = dict(out_norm="layer", out_weight=t["out_weight"], out_bias=t["out_bias"])
+    s, o = _rn().residual_norm(t["residual"], t["branch"], **kw)
+    assert torch.equal(o[1], t["out_bias"]) and torch.equal(s[1], torch.zeros_like(s[1]))
+    assert bool(torch.isnan(o[5:7]).all()) and bool(torch.isfinite(o[[0, 1, 2, 3, 4, 7]]).all())
+    empty = _rn().residual_norm(t["residual"][:0], t["branch"][:0], **kw)
+    assert empty[0].shape == (0, 768) and empty[1].shape == (0, 768)
+    d = _rn().residual_norm_backward(t["residual"][:0], t["residual"][:0], t["residual"][:0], t["branch"][:0], out_norm="layer", out_weight=t["out_weight"])
+    assert d["branch"].shape == (0, 768) and bool((d["out_weight"] == 0).all()) and bool((d["out_bias"] == 0).all())
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (5, 40), (3, 512), (4, 769), (2, 2048), (3, 8192)])
+def test_quantised_rows_of_the_norm(rows, cols):
+    from souffle_models_b200 import int8
+    t = _make(rows, cols, torch.float32, torch.float32, "none", "rms", 0)
+    kw = dict(out_norm="rms", out_weight=t["out_weight"])
+    o = _rn().residual_norm(t["residual"], t["branch"], **kw)[1]
+    _, (q, scale) = _rn().residual_norm(t["residual"], t["branch"], quantize=True, **kw)
+    want_q, want_scale = int8.quantize_rows(o)          # of the same fp32 values: bit for bit
+    assert torch.equal(q, want_q) and torch.equal(scale, want_scale)
+    with pytest.raises(ValueError):
+        _rn().residual_norm(t["residual"].requires_grad_(), t["branch"], quantize=True, **kw)
+
+
+# ---- gradients ---------------------------------------------------------------------------------------------------
+
+def _gradients64(t, n1, n2, alpha, beta, ds, do):
+    leaf = {k: v.double().requires_grad_() for k, v in t.items() if v is not None}
+    s, o = _formula({k: leaf.get(k) for k in t}, n1, n2, alpha, beta)
+    total = (s * ds.double()).sum() if ds is not None else 0
+    if o is not None:
+        total = total + (o * do.double()).sum()
+    return dict(zip(leaf, torch.autograd.grad(total, list(leaf.values()))))
+
+
+def _check_gradients(rows, cols, dtype, params, n1, n2, gates, seed=0, with_sum=True, residual=True):
+    t = _make(rows, cols, dtype, params, n1, n2, gates, seed, residual)
+    g = torch.Generator(device="cuda").manual_seed(seed + 1)
+    ds = torch.randn(rows, cols, generator=g, device="cuda").to(dtype) if with_sum or n2 == "none" else None
+    do = torch.randn(rows, cols, generator=g, device="cuda").to(dtype) if n2 != "none" else None
+    got = _rn().residual_norm_backward(ds, do, t["residual"], t["branch"], branch_norm=n1, branch_weight=t["branch_weight"],
+                                       branch_bias=t["branch_bias"], gate=t["gate"], out_norm=n2, out_weight=t["out_weight"], residual_scale=0.9,
+                                       branch_scale=1.25)
+    want = _gradients64(t, n1, n2, 0.9, 1.25, ds, do)
+    for k in t:
+        if k not in want:
+            assert got[k] is None, k
+            continue
+        # in norm: a row's gradient is a chain of two norms, each of which multiplies fp32's errors by at most its rows' largest
+        # normalised magnitude squared (< 6^2 here) times a few; small widths have deviations near zero, so the bound is by norm
+        norm = want[k].norm().item()
+        err = (got[k].double() - want[k]).norm().item()
+        assert got[k].shape == want[k].shape
+        assert err <= U[got[k].dtype] * norm + 512 * E32 * norm * max(1.0, 32 / cols) + 1e-30, (k, err / norm)
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 64), (2, 33), (5, 64), (17, 255), (300, 264), (1001, 513), (157, 768), (40, 1001), (700, 2048), (20, 4096),
+                                       (9, 4104), (150, 8192), (3, 8191)])
+@pytest.mark.parametrize("n1,n2", KINDS)
+def test_gradients_against_the_formula(rows, cols, n1, n2):
+    for k, (dtype, params) in enumerate(TYPES[::2]):
+        divisors = [d for d in range(2, rows + 1) if rows % d == 0]
+        _check_gradients(rows, cols, dtype, params, n1, n2, gates=(0, 1, divisors[len(divisors) // 2] if divisors else 1)[k], seed=k)
+
+
+@pytest.mark.parametrize("gates", [1, 2, 3, 7, 30, 70, 210, 2310])
+@pytest.mark.parametrize("cols", [96, 777])
+def test_gradients_of_gates_whatever_rows_share_one(gates, cols):
+    _check_gradients(2310, cols, torch.float32, torch.float32, "layer", "rms", gates)
+    _check_gradients(2310, cols, torch.bfloat16, torch.bfloat16, "none", "none", gates)
+
+
+@pytest.mark.parametrize("dtype,params", TYPES)
+def test_gradients_of_every_type_and_without_parts(dtype, params):
+    _check_gradients(130, 776, dtype, params, "layer", "layer", 13)
+    _check_gradients(130, 776, dtype, params, "rms", "layer", 0, with_sum=False, residual=False)
+
+
+def test_gradients_do_not_change_from_run_to_run():
+    t = _make(3000, 776, torch.float16, torch.float32, "layer", "layer", 10)
+    ds, do = torch.randn_like(t["branch"]), torch.randn_like(t["branch"])
+    kw = dict(branch_norm="layer", branch_weight=t["branch_weight"], branch_bias=t["branch_bias"], gate=t["gate"], out_norm="layer",
+              out_weight=t["out_weight"])
+    a, b = (_rn().residual_norm_backward(ds, do, t["residual"], t["branch"], **kw) for _ in range(2))
+    for k in a:
+        assert torch.equal(a[k], b[k]), k
+
+
+@pytest.mark.parametrize("n1,n2", [("layer", "layer"), ("rms", "rms"), ("none", "layer")])
+def test_gradients_against_differences(n1, n2):
+    """Central differences of the formula in 64 bits along random directions: their own error is h^2 / 6 times a third derivative, below
+    1e-7 of the slope's scale at h = 1e-4; the kernel's fp32 gradients add a few 1e-6."""
+    t = _make(12, 72, torch.float32, torch.float32, n1, n2, 4)
+    ds, do = torch.randn_like(t["branch"]), torch.randn_like(t["branch"])
+    got = _rn().residual_norm_backward(ds, do, t["residual"], t["branch"], branch_norm=n1, branch_weight=t["branch_weight"],
+                                       branch_bias=t["branch_bias"], gate=t["gate"], out_norm=n2, out_weight=t["out_weight"])
+
+    def value(k, v):
+        s, o = _formula({**{n: None if x is None else x.double() for n, x in t.items()}, k: v}, n1, n2, 1.0, 1.0)
+        return ((s * ds.double()).sum() + (o * do.double()).sum()).item()
+
+    for k, x in t.items():
+        if x is None:
+            continue
+        g = torch.Generator(device="cuda").manual_seed(len(k))
+        way = torch.randn(x.shape, generator=g, device="cuda", dtype=torch.float64)
+        slope = (value(k, x.double() + 1e-4 * way) - value(k, x.double() - 1e-4 * way)) / 2e-4
+        assert abs((got[k].double() * way).sum().item() - slope) <= 2e-5 * got[k].double().norm().item() * way.norm().item(), k
+
+
+def test_autograd_gives_the_same_gradients():
+    t = _make(24, 264, torch.float32, torch.float32, "layer", "rms", 6)
+    leaf = {k: v.clone().requires_grad_() for k, v in t.items() if v is not None}
+    kw = dict(branch_norm="layer", out_norm="rms", residual_scale=0.9)
+    s, o = _rn().residual_norm(leaf["residual"], leaf["branch"], branch_weight=leaf["branch_weight"], branch_bias=leaf["branch_bias"],
+                               gate=leaf["gate"], out_weight=leaf["out_weight"], **kw)
+    ds, do = torch.randn_like(s), torch.randn_like(o)
+    torch.autograd.backward((s, o), (ds, do))
+    want = _rn().residual_norm_backward(ds, do, t["residual"], t["branch"], branch_weight=t["branch_weight"], branch_bias=t["branch_bias"],
+                                        gate=t["gate"], out_weight=t["out_weight"], **kw)
+    for k, v in leaf.items():
+        assert torch.equal(v.grad, want[k]), k
+    for v in leaf.values():
+        v.grad = None
+    s, o = _rn().residual_norm(leaf["residual"], leaf["branch"], branch_weight=leaf["branch_weight"], branch_bias=leaf["branch_bias"],
+                               gate=leaf["gate"], out_weight=leaf["out_weight"], **kw)
+    s.sum().backward()                                   # the norm's output is not used
+    assert bool((leaf["out_weight"].grad == 0).all()) and bool(torch.allclose(leaf["residual"].grad, torch.full_like(s, 0.9)))
+
+
+def test_refusals():
+    rn = _rn().residual_norm
+    x = torch.zeros(4, 64, dtype=torch.float16, device="cuda")
+    v = torch.zeros(64, dtype=torch.float16, device="cuda")
+    from souffle_models_b200 import SouffleError
+    for bad in (dict(residual=x.float()), dict(residual=x[:2]), dict(branch=x.double(), residual=None), dict(branch=x.cpu(), residual=None),
+                dict(out_norm="batch"), dict(out_norm="layer", out_weight=v[:32]), dict(out_norm="layer", out_weight=v, out_bias=v.float()),
+                dict(gate=x[:3]), dict(gate=x[:, :32].contiguous()), dict(keep_sum=False), dict(branch=x.t(), residual=x.t()),
+                dict(out_norm="layer", out_weight=v.cpu())):
+        with pytest.raises(ValueError):
+            rn(**{**dict(residual=x, branch=x), **bad})
+    for bad in (dict(out_weight=v), dict(out_norm="rms", out_weight=v, out_bias=v), dict(out_norm="layer", out_eps=-1.0),
+                dict(out_norm="layer", out_weight=v.bfloat16()), dict(branch=x[:1].expand(4, 64))):
+        with pytest.raises(SouffleError):
+            rn(**{**dict(residual=x, branch=x), **bad})
+    wide = torch.zeros(1, 8200, dtype=torch.float16, device="cuda")
+    with pytest.raises(SouffleError):
+        rn(wide, wide)
+    with pytest.raises(SouffleError):
+        _rn().residual_norm_backward(x, None, x, x, out_norm="layer", out_weight=v)
+
+
+def test_on_another_stream_and_in_a_graph():
+    t = _make(64, 768, torch.float16, torch.float16, "none", "layer", 0)
+    kw = dict(out_norm="layer", out_weight=t["out_weight"], out_bias=t["out_bias"])
+    want = _rn().residual_norm(t["residual"], t["branch"], **kw)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _rn().residual_norm(t["residual"], t["branch"], **kw)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = _rn().residual_norm(t["residual"], t["branch"], **kw)
+    torch.cuda.current_stream().wait_stream(side)
+    graph.replay()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
