@@ -421,6 +421,9 @@ typedef struct SouffleInt8Linear {
 } SouffleInt8Linear;
 size_t souffle_int8_linear_workspace_bytes(int32_t rows, int32_t inner, int32_t x_dtype);
 int souffle_int8_linear_forward(const SouffleInt8Linear* call, souffle_stream_t stream);
+/* Blocks until `stream` is idle; SOUFFLE_DEVICE_TIMEOUT if, since the last such call on this device, a bounded wait of a product
+ * has run out (its output is then undefined). */
+int souffle_int8_linear_status(souffle_stream_t stream);
 
 /* Blocks until `stream` is idle, then decodes the status words in `workspace`. */
 int souffle_workspace_status(void* workspace, souffle_stream_t stream);

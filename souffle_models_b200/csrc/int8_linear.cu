@@ -148,6 +148,209 @@ __global__ void __launch_bounds__(32 * kFewWarps) souffle_int8_few(const LinearA
   }
 }
 
+// ---- many tokens -------------------------------------------------------------------------------------------------
+
+// A pair of CTAs computes tiles of 256 tokens x bn channels with pair MMAs of kind::i8: each CTA loads its own 128 rows of tokens and
+// half of the tile's channels, 128 bytes of the inner dimension at a time, and finds its 128 x bn sums in its own tensor memory.
+// Warp 0 feeds, warp 1 of the pair's leader issues the MMAs, warps 2-9 turn the sums of one tile into outputs while the next
+// tile's are computed in the other half of tensor memory.  Zeros past the matrices' ends come from the copy engine.
+constexpr int kPairThreads = 320, kPairStages = 5, kPairOperand = 128 * 128, kPairEpiWarps = 8, kPairBox = 2048, kPairMaxBn = 256;
+constexpr unsigned long long kPairTimeoutNs = 2000000000ull;
+struct PairCtl {
+  uint64_t full[kPairStages], empty[kPairStages], tmem_full[2], tmem_empty[2];
+  WaitCtl wait;
+  uint32_t tmem_base;
+  int abort;
+  float w_scale[2][kPairMaxBn], bias[2][kPairMaxBn];
+};
+constexpr int kPairRing = 2 * kPairStages * kPairOperand, kPairBoxes = 2 * kPairEpiWarps * kPairBox;
+constexpr int kPairSmem = kPairRing + kPairBoxes + (int)sizeof(PairCtl) + 1024;      // 1024: the base need not be aligned
+
+struct PairArgs {
+  CUtensorMap x, w, out;
+  LinearArgs a;
+  int bn, tiles_n, tiles, chunks;
+};
+
+// {code, where, cta, 0} of the first wait that ran out since the status was last read
+__device__ int g_linear_status[4];
+
+template <class T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) { return pack_h2(a, b); }
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// kBoxed: the outputs' rows begin on 16-byte boundaries, so that the copy engine can write them.
+template <class T, bool kBoxed>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) souffle_int8_pairs(const __grid_constant__ PairArgs p) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* base = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);       // the same in both CTAs: their windows begin alike
+  const uint32_t ring = smem_u32(base);
+  uint8_t* boxes = base + kPairRing;
+  PairCtl& cs = *reinterpret_cast<PairCtl*>(boxes + kPairBoxes);
+  const LinearArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_cta_rank();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kPairStages; ++i) {
+      mbar_init(smem_u32(&cs.full[i]), 1);
+      mbar_init(smem_u32(&cs.empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&cs.tmem_full[i]), 1);
+      mbar_init(smem_u32(&cs.tmem_empty[i]), 2 * kPairEpiWarps);
+    }
+    cs.abort = 0;
+    cs.wait.abort_smem = &cs.abort;
+    cs.wait.status_g = g_linear_status;
+    cs.wait.deadline_ns = globaltimer_ns() + kPairTimeoutNs;
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc_pair(smem_u32(&cs.tmem_base), 512);
+  if (warp == 0 && lane < 3) tma_prefetch_desc(lane == 0 ? &p.x : lane == 1 ? &p.w : &p.out);
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();                  // the peer's barriers exist before anything arrives on them
+  tc_fence_after_sync();
+  const uint32_t tmem = cs.tmem_base;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      const uint32_t half = (uint32_t)(p.bn >> 1) * 128u;
+      uint32_t s = 0, parity = 1;      // a slot that has never been used is empty
+      bool ok = true;
+      for (int t = first; ok && t < p.tiles; t += step) {
+        const int m0 = (t / p.tiles_n) * 256 + (int)rank * 128, n0 = (t % p.tiles_n) * p.bn + (int)rank * (p.bn >> 1);
+        for (int c = 0; c < p.chunks; ++c) {
+          if (!(ok = mbar_wait_hot(smem_u32(&cs.empty[s]), parity, cs.wait, 1))) break;
+          const uint32_t full = smem_u32(&cs.full[s]), at = ring + s * 2 * kPairOperand;
+          if (rank == 0) mbar_expect_tx(full, 2 * (kPairOperand + half));
+          const uint32_t leader = map_shared_rank(full, 0);
+          tma_load_2d_pair(at, &p.x, leader, c * 128, m0);
+          tma_load_2d_pair(at + kPairOperand, &p.w, leader, c * 128, n0);
+          if (++s == kPairStages) s = 0, parity ^= 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && elect_one()) {
+      const uint32_t idesc = umma_idesc_i8_pair((uint32_t)p.bn);
+      uint32_t s = 0, parity = 0, buf = 0, free_parity = 1;
+      bool ok = true;
+      for (int t = first; ok && t < p.tiles; t += step) {
+        if (!mbar_wait_hot(smem_u32(&cs.tmem_empty[buf]), free_parity, cs.wait, 2)) break;
+        tc_fence_after_sync();
+        for (int c = 0; c < p.chunks; ++c) {
+          if (!(ok = mbar_wait_hot(smem_u32(&cs.full[s]), parity, cs.wait, 3))) break;
+          tc_fence_after_sync();
+          const uint32_t at = ring + s * 2 * kPairOperand;
+          umma_i8_k128_pair(tmem + buf * 256, umma_desc_lo(at, 16), umma_desc_lo(at + kPairOperand, 16), idesc, c != 0);
+          umma_commit_pair(smem_u32(&cs.empty[s]));
+          if (++s == kPairStages) s = 0, parity ^= 1;
+        }
+        if (ok) umma_commit_pair(smem_u32(&cs.tmem_full[buf]));
+        if (buf ^= 1, buf == 0) free_parity ^= 1;
+      }
+    }
+  } else {
+    constexpr int kBoxCols = 64 / (int)sizeof(T);
+    const int quarter = warp & 3, part = (warp - 2) >> 2, tid = threadIdx.x - 64;
+    uint8_t* box = boxes + (warp - 2) * 2 * kPairBox;
+    uint32_t buf = 0, parity = 0, which = 0;
+    for (int t = first; t < p.tiles; t += step) {
+      const int m0 = (t / p.tiles_n) * 256 + (int)rank * 128 + quarter * 32, n0 = (t % p.tiles_n) * p.bn;
+      if (tid < p.bn) {
+        const int n = n0 + tid;
+        cs.w_scale[buf][tid] = n < a.cols ? a.w_scale[n] : 0.0f;
+        cs.bias[buf][tid] = a.bias && n < a.cols ? to_f32(static_cast<const T*>(a.bias)[n]) : 0.0f;
+      }
+      const float xs = m0 + lane < a.rows ? a.x_scale[m0 + lane] : 0.0f;
+      named_barrier_sync(1, 32 * kPairEpiWarps);
+      const bool ok = mbar_wait_warp(smem_u32(&cs.tmem_full[buf]), parity, cs.wait, 4, lane);
+      if (ok) {                        // (all warps go through the tiles and meet at their barriers, given up or not)
+        tc_fence_after_sync();
+        for (int c0 = 32 * part; c0 < p.bn; c0 += 64) {
+          uint32_t r[32];
+          tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + buf * 256 + c0, r);
+          tmem_ld_wait(r);
+          if (n0 + c0 >= a.cols) continue;
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 w = *reinterpret_cast<const float4*>(&cs.w_scale[buf][c0 + i]), b = *reinterpret_cast<const float4*>(&cs.bias[buf][c0 + i]);
+            v[i] = fmaf((float)(int)r[i] * xs, w.x, b.x);
+            v[i + 1] = fmaf((float)(int)r[i + 1] * xs, w.y, b.y);
+            v[i + 2] = fmaf((float)(int)r[i + 2] * xs, w.z, b.z);
+            v[i + 3] = fmaf((float)(int)r[i + 3] * xs, w.w, b.w);
+          }
+          if (a.act == SOUFFLE_ACT_RELU) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
+          } else if (a.act == SOUFFLE_ACT_GELU) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = gelu_sigmoid(v[i]);
+          }
+          uint32_t words[8 * sizeof(T)];
+          if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) words[i] = __float_as_uint(v[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) words[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+          }
+#pragma unroll
+          for (int b = 0; b < 32 / kBoxCols; ++b) {
+            uint8_t* at = box + which * kPairBox;
+            if (kBoxed) {
+              if (lane == 0) bulk_wait_group_read<1>();        // the box's last copy has read it
+              __syncwarp();
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)                          // the layout of a 64B-swizzled box
+              *reinterpret_cast<uint4*>(at + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
+                  make_uint4(words[16 * b + 4 * i], words[16 * b + 4 * i + 1], words[16 * b + 4 * i + 2], words[16 * b + 4 * i + 3]);
+            if (kBoxed) {
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                if (n0 + c0 + b * kBoxCols < a.cols && m0 < a.rows) tma_store_2d(&p.out, smem_u32(at), n0 + c0 + b * kBoxCols, m0);
+                bulk_commit_group();
+              }
+            } else {
+              __syncwarp();
+              const int c = lane % kBoxCols, n = n0 + c0 + b * kBoxCols + c;
+              for (int row = lane / kBoxCols; row < 32; row += 32 / kBoxCols) {
+                const T value = *reinterpret_cast<const T*>(at + row * 64 + ((((c * (int)sizeof(T)) >> 4) ^ ((row >> 1) & 3)) << 4) + ((c * (int)sizeof(T)) & 15));
+                if (n < a.cols && m0 + row < a.rows) static_cast<T*>(a.out)[(m0 + row) * a.out_stride + n] = value;
+              }
+              __syncwarp();
+            }
+            which ^= 1;
+          }
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_relaxed(map_shared_rank(smem_u32(&cs.tmem_empty[buf]), 0));
+      }
+      if (buf ^= 1, buf == 0) parity ^= 1;
+    }
+    if (kBoxed && lane == 0) bulk_wait_group_all();
+  }
+
+  __syncthreads();
+  if (cs.abort) {                      // copies that were issued already land before the shared memory is given up
+    const unsigned long long t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();                  // both CTAs are done with the pair's tensor memory and with each other's barriers
+  if (warp == 1) tmem_dealloc_pair(tmem, 512);
+}
+
 // ---- host --------------------------------------------------------------------------------------------------------
 
 static bool is_float_type(int t) { return t >= SOUFFLE_F32 && t <= SOUFFLE_BF16; }
@@ -174,6 +377,63 @@ static int quantise(const void* x, int dtype, long long x_stride, int rows, int 
   return quantise_launch(static_cast<const __nv_bfloat16*>(x), x_stride, rows, cols, q, q_stride, scale, st);
 }
 static long long padded16(long long n) { return (n + 15) / 16 * 16; }
+
+static int make_map(CUtensorMap* m, CUtensorMapDataType type, const void* p, uint64_t rows, uint64_t cols, uint64_t pitch_bytes, uint32_t box_cols,
+                    uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(SOUFFLE_CUDA_ERROR, "cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch_bytes};
+  const cuuint32_t box[2] = {box_cols, box_rows}, one[2] = {1, 1};
+  const CUresult r = fn(m, type, 2, const_cast<void*>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? SOUFFLE_OK : fail(SOUFFLE_CUDA_ERROR, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+}
+
+// The tile width that takes the fewest cycles: whole tiles dealt out to the pairs, each bound by its MMAs (bn / 2 cycles a step of
+// 32, 51 at least) or by its epilogue, the last one's epilogue behind everything.
+static int choose_bn(int rows, int inner, int cols, int act, int pairs) {
+  int best = 256;
+  double least = 1e30;
+  for (int bn = 256; bn >= 64; bn -= 64) {
+    const long long tiles = ((rows + 255) / 256) * (long long)((cols + bn - 1) / bn), waves = (tiles + pairs - 1) / pairs;
+    const double loop = ((inner + 127) / 128) * 4.0 * (bn / 2 > 51 ? bn / 2 : 51), epi = bn * (act == SOUFFLE_ACT_GELU ? 16.0 : 8.0);
+    const double cycles = waves * (loop > epi ? loop : epi) + epi;
+    if (cycles < least * 0.97) least = cycles, best = bn;
+  }
+  return best;
+}
+
+template <class T>
+static int pairs_launch(const LinearArgs& a, int sms, cudaStream_t st) {
+  PairArgs p;
+  p.a = a;
+  p.bn = choose_bn(a.rows, a.inner, a.cols, a.act, sms / 2);
+  p.tiles_n = (a.cols + p.bn - 1) / p.bn;
+  p.chunks = (a.inner + 127) / 128;
+  const long long tiles = (long long)((a.rows + 255) / 256) * p.tiles_n;
+  if (tiles > (1 << 30)) return fail(SOUFFLE_BAD_SHAPE, "8-bit product of %d x %d: too many tiles", a.rows, a.cols);
+  p.tiles = (int)tiles;
+  int rc;
+  if ((rc = make_map(&p.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.x, a.rows, a.inner, a.x_stride, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B)) ||
+      (rc = make_map(&p.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w, a.cols, a.inner, a.w_stride, 128, p.bn / 2, CU_TENSOR_MAP_SWIZZLE_128B)))
+    return rc;
+  const bool boxed = ((uintptr_t)a.out & 15u) == 0 && (a.out_stride * (long long)sizeof(T)) % 16 == 0;
+  if (boxed) {
+    const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+    if ((rc = make_map(&p.out, type, a.out, a.rows, a.cols, a.out_stride * sizeof(T), 64 / sizeof(T), 32, CU_TENSOR_MAP_SWIZZLE_64B))) return rc;
+  } else {
+    p.out = p.x;                       // a map that exists, for the prefetch
+  }
+  auto fn = boxed ? souffle_int8_pairs<T, true> : souffle_int8_pairs<T, false>;
+  SF_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+  const int pairs = p.tiles < sms / 2 ? p.tiles : sms / 2;
+  fn<<<2 * pairs, kPairThreads, kPairSmem, st>>>(p);
+  SF_CUDA(cudaGetLastError());
+  return SOUFFLE_OK;
+}
+
+// Rows from which on the tensor cores' fifth generation is used
+constexpr int kFewRows = 64;
 
 }  // namespace souffle
 
@@ -230,18 +490,23 @@ int souffle_int8_linear_forward(const SouffleInt8Linear* call, souffle_stream_t 
     if ((rc = quantise(d.x, d.x_dtype, d.x_stride, d.rows, d.inner, q, padded16(d.inner), scale, st))) return rc;
     a.x = q; a.x_scale = scale; a.x_stride = padded16(d.inner);
   }
-  const int ny = (d.rows + 15) / 16;
-  for (int y0 = 0; y0 < ny; y0 += 65535) {                 // a grid has at most 65535 rows of blocks
-    LinearArgs b = a;
-    b.x = static_cast<const signed char*>(a.x) + 16LL * y0 * a.x_stride;
-    b.x_scale = a.x_scale + 16LL * y0;
-    b.out = static_cast<char*>(a.out) + 16LL * y0 * a.out_stride * (long long)oe;
-    b.rows = a.rows - 16 * y0;
-    const int n = ny - y0 < 65535 ? ny - y0 : 65535;
-    souffle_int8_few<2><<<dim3((d.cols + 15) / 16, n), 32 * kFewWarps, 0, st>>>(b);
-    SF_CUDA(cudaGetLastError());
+  if (d.rows > kFewRows) {
+    if (d.out_dtype == SOUFFLE_F32) return pairs_launch<float>(a, sms, st);
+    return d.out_dtype == SOUFFLE_F16 ? pairs_launch<__half>(a, sms, st) : pairs_launch<__nv_bfloat16>(a, sms, st);
   }
+  souffle_int8_few<2><<<dim3((d.cols + 15) / 16, (d.rows + 15) / 16), 32 * kFewWarps, 0, st>>>(a);
+  SF_CUDA(cudaGetLastError());
   return SOUFFLE_OK;
+}
+
+int souffle_int8_linear_status(souffle_stream_t stream) {
+  SF_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
+  int h[4];
+  SF_CUDA(cudaMemcpyFromSymbol(h, g_linear_status, sizeof(h)));
+  if (h[0] == 0) return SOUFFLE_OK;
+  const int clear[4] = {0, 0, 0, 0};
+  SF_CUDA(cudaMemcpyToSymbol(g_linear_status, clear, sizeof(clear)));
+  return fail(SOUFFLE_DEVICE_TIMEOUT, "8-bit product: device wait expired (code %d, where %d, cta %d)", h[0], h[1], h[2]);
 }
 
 }  // extern "C"

@@ -319,6 +319,27 @@ __device__ __forceinline__ void umma_f16_k64_pair(uint32_t d_tmem, uint32_t a_lo
       ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(bstep), "r"(idesc), "r"(acc0), "r"(kDescHiSw128)
       : "memory");
 }
+// kind::i8, signed 8-bit x signed 8-bit -> 32-bit integers, both operands K-major: [4,6) D format (2 = s32), [7,10) and [10,13) A and B
+// (1 = signed).  N a multiple of 32.
+__device__ __forceinline__ uint32_t umma_idesc_i8_pair(uint32_t n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((256u >> 4) << 24);
+}
+// One K chunk of 128 bytes as four pair MMAs of 32.
+__device__ __forceinline__ void umma_i8_k128_pair(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc0) {
+  asm volatile(
+      "{\n\t.reg .pred p, pt;\n\t.reg .b64 da, db;\n\t.reg .b32 al, bl;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 pt, 0, 0;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %3, p;\n\t"
+      "add.u32 al, %1, 2;\n\tadd.u32 bl, %2, 2;\n\tmov.b64 da, {al, %5};\n\tmov.b64 db, {bl, %5};\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %3, pt;\n\t"
+      "add.u32 al, al, 2;\n\tadd.u32 bl, bl, 2;\n\tmov.b64 da, {al, %5};\n\tmov.b64 db, {bl, %5};\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %3, pt;\n\t"
+      "add.u32 al, al, 2;\n\tadd.u32 bl, bl, 2;\n\tmov.b64 da, {al, %5};\n\tmov.b64 db, {bl, %5};\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %3, pt;\n\t}"
+      ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(acc0), "r"(kDescHiSw128)
+      : "memory");
+}
 // Arrives, once every pair MMA issued so far by this thread has completed, on the mbarrier at this shared-memory
 // offset in BOTH CTAs of the pair (the commit is multicast over the cluster; it carries no data).
 __device__ __forceinline__ void umma_commit_pair(uint32_t bar) {

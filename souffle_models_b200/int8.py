@@ -88,6 +88,11 @@ def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: O
     return out
 
 
+def status() -> None:
+    """Synchronises the current stream and raises SouffleError if a device-side wait of a product has expired."""
+    _lib.check(_lib.load().souffle_int8_linear_status(_lib.stream_ptr()))
+
+
 class Int8Mlp:
     """The MLP half of an encoder layer on 8-bit products, from the fp16 weights that BertEncoder and SwinBlock take (fc1_w [C, F],
     fc2_w [F, C], optional biases fc1_b, fc2_b and the norm's weight and bias):
