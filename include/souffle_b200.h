@@ -354,7 +354,7 @@ int souffle_se_module_forward(const float* input, const float* w_reduce, const f
 enum { SOUFFLE_F32 = 0, SOUFFLE_F16 = 1, SOUFFLE_BF16 = 2 };
 enum { SOUFFLE_NORM_NONE = 0, SOUFFLE_NORM_LAYER = 1, SOUFFLE_NORM_RMS = 2 };
 typedef struct SouffleResidualNorm {
-  int32_t rows, cols;        /* rows >= 0, 1 <= cols <= 8192 */
+  int32_t rows, cols;        /* 0 <= rows <= 2^30, 1 <= cols <= 8192 */
   int32_t dtype;             /* of residual, branch, sum, out: SOUFFLE_F32, _F16 or _BF16 */
   int32_t param_dtype;       /* of gate, weights and biases: the same, or SOUFFLE_F32 */
   int32_t branch_norm, out_norm;
@@ -391,6 +391,9 @@ typedef struct SouffleResidualNormGrad {
 } SouffleResidualNormGrad;
 size_t souffle_residual_norm_backward_workspace_bytes(int32_t rows, int32_t cols, int32_t gate_rows);
 int souffle_residual_norm_backward(const SouffleResidualNormGrad* call, souffle_stream_t stream);
+/* Blocks until `stream` is idle; SOUFFLE_DEVICE_TIMEOUT if, since the last such call on this device, a bounded wait of one of these
+ * calls has run out (its results are then undefined). */
+int souffle_residual_norm_status(souffle_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
  * Products in 8-bit integers with a scale per token and one per channel (no counterpart in the reference).

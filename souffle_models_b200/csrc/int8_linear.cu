@@ -37,9 +37,9 @@ __global__ void __launch_bounds__(256) souffle_quantise_rows(const T* __restrict
   Team team;
   team.begin(box, warps_per_row, warp % warps_per_row, 1, cols, 0);
   if (kGroups * 256 * warps_per_row >= cols_n) {
-    float v[kGroups][8];
+    F8 v[kGroups];
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i) cols.load(from, i, v[i]);
+    for (int i = 0; i < kGroups; ++i) v[i] = cols.load(from, i);
     quantise_row<kGroups>(team, cols, v, to, scale + row);
     return;
   }
@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(256) souffle_quantise_rows(const T* __restrict
   const int groups = (cols_n + 256 * warps_per_row - 1) / (256 * warps_per_row);
   for (int i = 0; i < groups; ++i) {
     float v[8];
-    cols.load(from, i, v);
+    unpack8(cols.load(from, i), v);
 #pragma unroll
     for (int j = 0; j < 8; ++j) most = max(most, abs_bits(v[j]));
   }
@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(256) souffle_quantise_rows(const T* __restrict
   const bool fine = most < 0x7f800000u;
   for (int i = 0; i < groups; ++i) {
     float v[8];
-    cols.load(from, i, v);
+    unpack8(cols.load(from, i), v);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (cols.has(i, j)) to[cols.at(i, j)] = (signed char)__float2int_rn(fine ? v[j] * rs.inv : 0.0f);

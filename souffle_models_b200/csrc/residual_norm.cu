@@ -8,6 +8,7 @@
 
 #include "host_common.h"
 #include "row_io.cuh"
+#include "sm100_ptx.cuh"
 
 namespace souffle {
 
@@ -19,13 +20,43 @@ struct NormArgs {
   void *s, *o;
   signed char* q;
   float* q_scale;
+  int param_dtype;
 };
+
+// group i of a vector of weights, biases or gates, whose type only the host knows
+template <bool kVec> __device__ __forceinline__ F8 load_param(const Columns<kVec>& cols, const NormArgs& a, const void* p, long long row, int i) {
+  if (a.param_dtype == SOUFFLE_F32) return cols.load(static_cast<const float*>(p) + row * a.cols, i);
+  if (a.param_dtype == SOUFFLE_F16) return cols.load(static_cast<const __half*>(p) + row * a.cols, i);
+  return cols.load(static_cast<const __nv_bfloat16*>(p) + row * a.cols, i);
+}
+template <bool kVec> __device__ __forceinline__ void store_param(const Columns<kVec>& cols, const NormArgs& a, void* p, long long row, const F8& v) {
+  if (a.param_dtype == SOUFFLE_F32) cols.store(static_cast<float*>(p) + row * a.cols, 0, v);
+  else if (a.param_dtype == SOUFFLE_F16) cols.store(static_cast<__half*>(p) + row * a.cols, 0, v);
+  else cols.store(static_cast<__nv_bfloat16*>(p) + row * a.cols, 0, v);
+}
+__device__ __forceinline__ float param_at(const NormArgs& a, const void* p, long long i) {
+  return a.param_dtype == SOUFFLE_F32 ? static_cast<const float*>(p)[i] : a.param_dtype == SOUFFLE_F16 ? to_f32(static_cast<const __half*>(p)[i])
+                                                                                                  : to_f32(static_cast<const __nv_bfloat16*>(p)[i]);
+}
 
 // Rows of a gate: row m takes gate row m / (rows / gate_rows).
 __device__ __forceinline__ int gate_row(const NormArgs& a, int row) { return row / (a.rows / a.gate_rows); }
 
-template <class T, class P, bool kVec, int kGroups>
-__global__ void __launch_bounds__(256) souffle_residual_norm(const NormArgs a, int warps_per_row) {
+// (x - mean) / deviation * weight + bias
+template <int kGroups, bool kVec>
+__device__ __forceinline__ void normalise(const Columns<kVec>& cols, const NormArgs& a, F8 (&x)[kGroups], float2 stats, const void* weight, const void* bias) {
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) {
+    x[i] = mul8(add8(x[i], -stats.x), stats.y);
+    if (weight) x[i] = mul8(x[i], load_param(cols, a, weight, 0, i));
+    if (bias) x[i] = add8(x[i], load_param(cols, a, bias, 0, i));
+  }
+}
+
+// The general form: any width, address and stride, a row per team and launch; columns read one by one.
+template <class T, int kGroups>
+__global__ void __launch_bounds__(256) souffle_residual_norm_any(const NormArgs a, int warps_per_row) {
+  constexpr bool kVec = false;
   __shared__ __align__(16) char box[kTeamBox];
   const int teams = blockDim.x / (32 * warps_per_row), warp = threadIdx.x >> 5;
   const int row = blockIdx.x * teams + warp / warps_per_row;       // several teams only where a team is one warp
@@ -34,51 +65,27 @@ __global__ void __launch_bounds__(256) souffle_residual_norm(const NormArgs a, i
   Team team;
   team.begin(box, warps_per_row, warp % warps_per_row, 1, cols, kGroups);
 
-  float u[kGroups][8], h[kGroups][8], v[8];
+  F8 u[kGroups], h[kGroups];
   const T* y = static_cast<const T*>(a.y) + row * a.y_stride;
 #pragma unroll
-  for (int i = 0; i < kGroups; ++i) cols.load(y, i, u[i]);
+  for (int i = 0; i < kGroups; ++i) u[i] = cols.load(y, i);
   if (a.r) {
     const T* r = static_cast<const T*>(a.r) + row * a.r_stride;
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i) cols.load(r, i, h[i]);
+    for (int i = 0; i < kGroups; ++i) h[i] = mul8(cols.load(r, i), a.alpha);
   } else {
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) h[i][j] = 0.0f;
+    for (int i = 0; i < kGroups; ++i) h[i] = all8(0.0f);
   }
   if (a.branch_norm != SOUFFLE_NORM_NONE) {
     const float2 st = row_stats<kGroups>(team, cols, u, a.branch_norm == SOUFFLE_NORM_RMS, a.eps1);
-#pragma unroll
-    for (int i = 0; i < kGroups; ++i) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) u[i][j] = (u[i][j] - st.x) * st.y;
-      if (a.w1) {
-        cols.load(static_cast<const P*>(a.w1), i, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) u[i][j] *= v[j];
-      }
-      if (a.b1) {
-        cols.load(static_cast<const P*>(a.b1), i, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) u[i][j] += v[j];
-      }
-    }
-  }
-  if (a.gate) {
-    const P* g = static_cast<const P*>(a.gate) + (long long)gate_row(a, row) * a.cols;
-#pragma unroll
-    for (int i = 0; i < kGroups; ++i) {
-      cols.load(g, i, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) u[i][j] *= v[j];
-    }
+    normalise<kGroups>(cols, a, u, st, a.w1, a.b1);
   }
 #pragma unroll
-  for (int i = 0; i < kGroups; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) h[i][j] = cols.has(i, j) ? fmaf(a.alpha, h[i][j], a.beta * u[i][j]) : 0.0f;
+  for (int i = 0; i < kGroups; ++i) {
+    if (a.gate) u[i] = mul8(u[i], load_param(cols, a, a.gate, gate_row(a, row), i));
+    h[i] = cols.mask(i, fma8(u[i], a.beta * cols.in(i), h[i]));
+  }
   if (a.s) {
     T* s = static_cast<T*>(a.s) + row * a.s_stride;
 #pragma unroll
@@ -86,27 +93,229 @@ __global__ void __launch_bounds__(256) souffle_residual_norm(const NormArgs a, i
   }
   if (a.out_norm == SOUFFLE_NORM_NONE) return;
   const float2 st = row_stats<kGroups>(team, cols, h, a.out_norm == SOUFFLE_NORM_RMS, a.eps2);
-#pragma unroll
-  for (int i = 0; i < kGroups; ++i) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) h[i][j] = (h[i][j] - st.x) * st.y;
-    if (a.w2) {
-      cols.load(static_cast<const P*>(a.w2), i, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) h[i][j] *= v[j];
-    }
-    if (a.b2) {
-      cols.load(static_cast<const P*>(a.b2), i, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) h[i][j] += v[j];
-    }
-  }
+  normalise<kGroups>(cols, a, h, st, a.w2, a.b2);
   if (a.o) {
     T* o = static_cast<T*>(a.o) + row * a.o_stride;
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) cols.store(o, i, h[i]);
   }
   if (a.q) quantise_row<kGroups>(team, cols, h, a.q + row * a.q_stride, a.q_scale + row);
+}
+
+// ---- rows through a ring in shared memory ------------------------------------------------------------------------
+// Where rows can be copied 16 bytes at a time, a team keeps the next few rows on their way: one lane asks for a row's operands by bulk
+// copies into the team's ring, which count on the slot's barrier, and the row's turn begins with a wait that is over by then.  Weights
+// and biases lie in shared memory as fp32 (ones and zeros where there are none, so that a row meets no branch for them), and so does
+// the team's gate, times the branch's scale.  A team is as few warps as can hold a row with 8 kGroups columns a lane.
+
+constexpr unsigned long long kRowTimeoutNs = 2000000000ull;
+constexpr int kMaxRowSlots = 4;
+// {code, where, cta, 0} of the first wait that ran out since the status was last read
+__device__ int g_norm_status[4];
+
+struct RowCtl {
+  WaitCtl wait;
+  int abort;
+};
+
+// Vectors in shared memory, in blocks of 256 columns: of each eight columns the first four in the block's first half, the others in the
+// second, so that neighbouring lanes read neighbouring 16 bytes.
+__host__ __device__ inline int plane_floats(int cols) { return (cols + 255) / 256 * 256; }
+__device__ __forceinline__ int plane_at(int c) { return (c & ~255) + ((c & 255) >> 1); }        // c a multiple of 8
+__device__ __forceinline__ F8 read_plane(const float* at) {
+  const ulonglong2 lo = *reinterpret_cast<const ulonglong2*>(at), hi = *reinterpret_cast<const ulonglong2*>(at + 128);
+  return {{lo.x, lo.y, hi.x, hi.y}};
+}
+__device__ __forceinline__ void write_plane(float* at, const F8& x) {
+  *reinterpret_cast<ulonglong2*>(at) = make_ulonglong2(x.p[0], x.p[1]);
+  *reinterpret_cast<ulonglong2*>(at + 128) = make_ulonglong2(x.p[2], x.p[3]);
+}
+// eight values of a vector of the call, whose type only the host knows
+__device__ __forceinline__ F8 read_param(const NormArgs& a, const void* p, long long at) {
+  if (a.param_dtype == SOUFFLE_F32) return expand(read16(static_cast<const float*>(p) + at));
+  if (a.param_dtype == SOUFFLE_F16) return expand(read16(static_cast<const __half*>(p) + at));
+  return expand(read16(static_cast<const __nv_bfloat16*>(p) + at));
+}
+
+// What the host lays out for a launch of these kernels.
+struct RowPlan {
+  int warps, teams, total_teams, slots;        // of a row; of a CTA; of the grid; of a team's ring
+  int row_bytes, operands;                     // of one operand's row; operands of a row in the ring
+  int team_bytes, vectors;                     // shared memory of a team; where the vectors begin
+};
+// shared memory: RowCtl (64 bytes), then each team's box, barriers, gate and ring, then the vectors
+__host__ __device__ inline int team_gate_at() { return kTeamBox + kMaxRowSlots * 8; }
+__host__ __device__ inline int team_ring_at(int cols, bool gate) { return team_gate_at() + (gate ? plane_floats(cols) * 4 : 0); }
+
+// A team's ring.  Operand k of the row in the current slot is read by at(k), the next row asked for once release() has been called by all.
+template <int kOperands> struct RowRing {
+  const char* from[kOperands];                 // of the row that is asked for next; null: no such operand
+  long long step[kOperands];                   // bytes from one asked row to the next
+  char* at0;
+  uint32_t bars, parity;
+  int slots, row_bytes, operands, slot, left;  // left: rows not yet asked for
+  __device__ __forceinline__ void ask(int s) { // one lane
+    const uint32_t bar = bars + 8 * s;
+    uint32_t to = smem_u32(at0) + s * operands * row_bytes;
+    mbar_expect_tx(bar, operands * row_bytes);
+#pragma unroll
+    for (int k = 0; k < kOperands; ++k)
+      if (from[k]) {
+        bulk_load(to, from[k], row_bytes, bar);
+        to += row_bytes;
+        from[k] += step[k];
+      }
+    --left;
+  }
+  // one lane: the barriers, and the first rows
+  __device__ __forceinline__ void begin() {
+    for (int i = 0; i < slots; ++i) mbar_init(bars + 8 * i, 1);
+    fence_mbar_init();
+    fence_proxy_async_smem();
+    for (int i = 0; i < slots && left > 0; ++i) ask(i);
+  }
+  __device__ __forceinline__ const char* wait(const WaitCtl& c) {
+    mbar_wait_hot(bars + 8 * slot, parity, c, 1);
+    return at0 + slot * operands * row_bytes;
+  }
+  __device__ __forceinline__ void release(bool lane) {      // behind a barrier of those that have read the slot
+    if (lane && left > 0) ask(slot);
+    if (++slot == slots) slot = 0, parity ^= 1;
+  }
+};
+
+__device__ __forceinline__ void row_ctl_begin(RowCtl& ctl) {
+  if (threadIdx.x == 0) {
+    ctl.abort = 0;
+    ctl.wait.abort_smem = &ctl.abort;
+    ctl.wait.status_g = g_norm_status;
+    ctl.wait.deadline_ns = globaltimer_ns() + kRowTimeoutNs;
+  }
+}
+__device__ __forceinline__ void row_ctl_end(const RowCtl& ctl) {
+  if (*const_cast<volatile int*>(&ctl.abort)) {        // copies that were issued already land before the shared memory is given up
+    const unsigned long long t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+  }
+}
+// kVectors vectors of the call, ones and zeros in turn where there are none, laid down for all teams.
+template <int kVectors> __device__ __forceinline__ void lay_vectors(float* to, const NormArgs& a, const void* const (&from)[kVectors]) {
+  for (int v = threadIdx.x; v < a.cols >> 3; v += blockDim.x) {
+    F8 x[kVectors];
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k) x[k] = from[k] ? read_param(a, from[k], 8 * v) : all8(k & 1 ? 0.0f : 1.0f);
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k) write_plane(to + k * plane_floats(a.cols) + plane_at(8 * v), x[k]);
+  }
+}
+
+template <class T, bool kFull, int kGroups, bool kN1>
+__global__ void __launch_bounds__(768, 1) souffle_residual_norm_rows(const NormArgs a, const RowPlan p) {
+  extern __shared__ __align__(128) char smem[];
+  RowCtl& ctl = *reinterpret_cast<RowCtl*>(smem);
+  const int warp = threadIdx.x >> 5, mine = warp / p.warps, t = threadIdx.x - mine * 32 * p.warps;
+  const int id = blockIdx.x * p.teams + mine, n = a.cols;
+  char* own = smem + 64 + mine * p.team_bytes;
+  const int warp_of = warp - mine * p.warps;
+  const WarpColumns cols = {256 * kGroups * warp_of + 8 * (t & 31), n};
+  float* gate_s = reinterpret_cast<float*>(own + team_gate_at()) + plane_at(cols.first);
+  const float *vec = reinterpret_cast<const float*>(smem + p.vectors), *vec_s = vec + plane_at(cols.first);
+  const bool have_r = a.r != nullptr, have_gate = a.gate != nullptr;
+  RowRing<2> ring;
+  ring.step[0] = p.total_teams * a.y_stride * (long long)sizeof(T);
+  ring.step[1] = p.total_teams * a.r_stride * (long long)sizeof(T);
+  ring.from[0] = static_cast<const char*>(a.y) + id * a.y_stride * (long long)sizeof(T);
+  ring.from[1] = have_r ? static_cast<const char*>(a.r) + id * a.r_stride * (long long)sizeof(T) : nullptr;
+  ring.at0 = own + team_ring_at(n, have_gate);
+  ring.bars = smem_u32(own + kTeamBox);
+  ring.parity = 0;
+  ring.slots = p.slots, ring.row_bytes = p.row_bytes, ring.operands = p.operands, ring.slot = 0;
+  ring.left = id < a.rows ? (a.rows - 1 - id) / p.total_teams + 1 : 0;
+  if (t == 0) ring.begin();
+  row_ctl_begin(ctl);
+  if (kN1) lay_vectors<4>(const_cast<float*>(vec), a, {a.w2, a.b2, a.w1, a.b1});
+  else lay_vectors<2>(const_cast<float*>(vec), a, {a.w2, a.b2});
+  const int plane = plane_floats(n);
+  Team team;
+  team.begin(own, p.warps, warp_of, 1 + mine, cols, kGroups);
+  __syncthreads();
+
+  auto has = [&](int i) { return kFull || cols.has(i, 0); };
+  auto norm = [&](F8 (&x)[kGroups], bool rms, float eps, const float* w, const float* b) {
+    float mean_w = 0.0f, m2 = 0.0f;
+    if (!rms) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) sum += sum8(x[i]);
+      mean_w = warp_total(sum) * team.inv_warp_cols;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) x[i] = add8(x[i], has(i) ? -mean_w : 0.0f);
+    }
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) m2 += dot8(x[i], x[i]);
+    m2 = warp_total(m2);
+    if (team.warps > 1) {
+      const float4 st = team.merge(mean_w, m2);
+      m2 = st.y;
+      if (!rms) {
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i) x[i] = add8(x[i], has(i) ? mean_w - st.x : 0.0f);
+      }
+    }
+    const float rstd = rsqrtf(m2 * team.inv_cols + eps);
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i)
+      if (has(i)) x[i] = fma8(mul8(x[i], rstd), read_plane(w + 256 * i), read_plane(b + 256 * i));
+  };
+
+  const int per_gate = have_gate ? a.rows / a.gate_rows : 0;
+  int gate_end = 0;                            // rows below it have the gate that is in shared memory
+  for (int row = id; row < a.rows; row += p.total_teams) {
+    if (have_gate && row >= gate_end) {        // every thread brings the columns that it will read
+      const int at = row / per_gate;
+      gate_end = (at + 1) * per_gate;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i)
+        if (has(i)) write_plane(gate_s + 256 * i, mul8(read_param(a, a.gate, (long long)at * n + cols.at(i, 0)), a.beta));
+    }
+    const T* slot = reinterpret_cast<const T*>(ring.wait(ctl.wait)) + cols.first;
+    F8 x[kGroups];
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) x[i] = has(i) ? expand(read16(slot + 256 * i)) : all8(0.0f);
+    if (kN1) norm(x, a.branch_norm == SOUFFLE_NORM_RMS, a.eps1, vec_s + 2 * plane, vec_s + 3 * plane);
+    if (have_gate) {
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i)
+        if (has(i)) x[i] = mul8(x[i], read_plane(gate_s + 256 * i));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) x[i] = mul8(x[i], a.beta);
+    }
+    if (have_r) {
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i)
+        if (has(i)) x[i] = fma8(expand(read16(slot + n + 256 * i)), a.alpha, x[i]);
+    }
+    if (team.warps == 1) __syncwarp();
+    else team.meet();
+    ring.release(t == 0);
+    if (a.s) {
+      T* s = static_cast<T*>(a.s) + row * a.s_stride + cols.first;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i)
+        if (has(i)) write16(s + 256 * i, narrow<T>(x[i]));
+    }
+    if (a.out_norm == SOUFFLE_NORM_NONE) continue;
+    norm(x, a.out_norm == SOUFFLE_NORM_RMS, a.eps2, vec_s, vec_s + plane);
+    if (a.o) {
+      T* o = static_cast<T*>(a.o) + row * a.o_stride + cols.first;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i)
+        if (has(i)) write16(o + 256 * i, narrow<T>(x[i]));
+    }
+    if (a.q) quantise_row<kGroups>(team, cols, x, a.q + row * a.q_stride, a.q_scale + row);
+  }
+  row_ctl_end(ctl);
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------
@@ -129,9 +338,10 @@ struct NormGradArgs {
 
 __device__ __forceinline__ int first_row(long long team, int rows, int teams) { return (int)(team * rows / teams); }
 
+constexpr int kGradWarps = 12;
 // kSharedSums: the sums lie in shared memory, [SUMS][8][threads], where 1024 threads leave no registers for them.
-template <class T, class P, bool kVec, bool kSharedSums>
-__global__ void __launch_bounds__(kSharedSums ? 1024 : 512) souffle_residual_norm_grad(const NormGradArgs g, int warps_per_row) {
+template <class T, bool kVec, bool kSharedSums>
+__global__ void __launch_bounds__(kSharedSums ? 1024 : 32 * kGradWarps, 1) souffle_residual_norm_grad(const NormGradArgs g, int warps_per_row) {
   extern __shared__ __align__(16) char smem[];
   const NormArgs& a = g.f;
   const int teams = blockDim.x / (32 * warps_per_row), warp = threadIdx.x >> 5, mine = warp / warps_per_row;
@@ -140,175 +350,312 @@ __global__ void __launch_bounds__(kSharedSums ? 1024 : 512) souffle_residual_nor
   Team team;
   team.begin(smem + mine * kTeamBox, warps_per_row, warp % warps_per_row, 1 + mine, cols, 1);
   float* sums = reinterpret_cast<float*>(smem + teams * kTeamBox);
+  const float in = cols.in(0);
 
-  float acc[SUMS][8];
+  F8 acc[SUMS];
 #pragma unroll
-  for (int k = 0; k < SUMS; ++k)
+  for (int k = 0; k < SUMS; ++k) {
+    acc[k] = all8(0.0f);
+    if (kSharedSums)
+      for (int j = 0; j < 8; ++j) sums[(k * 8 + j) * blockDim.x + threadIdx.x] = 0.0f;
+  }
+  auto add = [&](int k, const F8& x, const F8& y) {       // += x y
+    if (kSharedSums) {
+      float v[8];
+      unpack8(mul8(x, y), v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (kSharedSums) sums[(k * 8 + j) * blockDim.x + threadIdx.x] = 0.0f;
-      else acc[k][j] = 0.0f;
+      for (int j = 0; j < 8; ++j) sums[(k * 8 + j) * blockDim.x + threadIdx.x] += v[j];
+    } else {
+      acc[k] = fma8(x, y, acc[k]);
     }
-  auto add = [&](int k, int j, float v) {
-    if (kSharedSums) sums[(k * 8 + j) * blockDim.x + threadIdx.x] += v;
-    else acc[k][j] += v;
   };
-  auto take = [&](int k, float (&v)[8], bool clear) {
+  auto add1 = [&](int k, const F8& x) {                   // += x
+    if (kSharedSums) {
+      float v[8];
+      unpack8(x, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sums[(k * 8 + j) * blockDim.x + threadIdx.x] += v[j];
+    } else {
+      acc[k] = add8(acc[k], x);
+    }
+  };
+  auto take = [&](int k) {                                // the sum, which begins anew
+    const F8 got = acc[k];
+    acc[k] = all8(0.0f);
+    if (!kSharedSums) return got;
+    float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      float& at = kSharedSums ? sums[(k * 8 + j) * blockDim.x + threadIdx.x] : acc[k][j];
+      float& at = sums[(k * 8 + j) * blockDim.x + threadIdx.x];
       v[j] = at;
-      if (clear) at = 0.0f;
+      at = 0.0f;
     }
+    return pack8(v);
   };
 
   const int begin = first_row(id, a.rows, g.teams), end = first_row(id + 1LL, a.rows, g.teams);
-  const int per_gate = a.gate ? a.rows / a.gate_rows : 0;
+  const int per_gate = a.gate ? a.rows / a.gate_rows : 0x7fffffff;
+  int gate_at = a.gate ? begin / per_gate : 0, gate_first = gate_at * per_gate;       // the row's gate, and that one's first row
   const bool n1 = a.branch_norm != SOUFFLE_NORM_NONE, n2 = a.out_norm != SOUFFLE_NORM_NONE;
+  const bool rms1 = a.branch_norm == SOUFFLE_NORM_RMS, rms2 = a.out_norm == SOUFFLE_NORM_RMS;
+  const T *yp = static_cast<const T*>(a.y) + begin * a.y_stride, *rp = static_cast<const T*>(a.r) + (a.r ? begin * a.r_stride : 0);
+  Eight<T> y_raw = zeros<T>(), r_raw = zeros<T>();
+  if (begin < end) {
+    y_raw = cols.fetch(yp, 0);
+    if (a.r) r_raw = cols.fetch(rp, 0);
+  }
   for (int row = begin; row < end; ++row) {
-    float y[8], h[8], d[8], e[8], w[8], gate[8];
-    cols.load(static_cast<const T*>(a.y) + row * a.y_stride, 0, y);
-    if (a.r) {
-      cols.load(static_cast<const T*>(a.r) + row * a.r_stride, 0, h);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) h[j] = 0.0f;
+    F8 y = expand(y_raw), h = expand(r_raw), u = y;
+    Eight<T> s_raw = zeros<T>(), o_raw = zeros<T>();
+    F8 gate = all8(1.0f);
+    if (a.gate) gate = load_param(cols, a, a.gate, gate_at, 0);
+    if (n2) o_raw = cols.fetch(static_cast<const T*>(g.dout) + row * g.do_stride, 0);
+    if (g.ds) s_raw = cols.fetch(static_cast<const T*>(g.ds) + row * g.ds_stride, 0);
+    if (row + 1 < end) {               // the next row's are on their way meanwhile
+      yp += a.y_stride;
+      y_raw = cols.fetch(yp, 0);
+      if (a.r) r_raw = cols.fetch(rp += a.r_stride, 0);
     }
-    if (g.ds) {
-      cols.load(static_cast<const T*>(g.ds) + row * g.ds_stride, 0, d);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) d[j] = 0.0f;
-    }
-    if (n2) cols.load(static_cast<const T*>(g.dout) + row * g.do_stride, 0, e);
-    if (a.gate) {
-      cols.load(static_cast<const P*>(a.gate) + (long long)(row / per_gate) * a.cols, 0, gate);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) gate[j] = 1.0f;
-    }
-    float u[8], rstd1 = 1.0f;
+    float rstd1 = 1.0f;
     if (n1) {                          // y becomes yhat, u = N1(y)
-      float (&y1)[1][8] = *reinterpret_cast<float (*)[1][8]>(&y);
-      const float2 st = row_stats<1>(team, cols, y1, a.branch_norm == SOUFFLE_NORM_RMS, a.eps1);
-      rstd1 = st.y;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) u[j] = y[j] = cols.has(0, j) ? (y[j] - st.x) * st.y : 0.0f;
-      if (a.w1) {
-        cols.load(static_cast<const P*>(a.w1), 0, w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) u[j] *= w[j];
-      }
-      if (a.b1) {
-        cols.load(static_cast<const P*>(a.b1), 0, w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) u[j] += w[j];
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) u[j] = y[j];
+      const float mean_w = rms1 ? 0.0f : warp_total(sum8(y)) * team.inv_warp_cols;
+      y = cols.mask(0, add8(y, -mean_w * in));
+      const float4 st = team.merge(mean_w, warp_total(dot8(y, y)));
+      rstd1 = rsqrtf(st.y * team.inv_cols + a.eps1);
+      if (team.warps > 1 && !rms1) y = cols.mask(0, add8(y, (mean_w - st.x) * in));
+      y = mul8(y, rstd1);
+      u = a.w1 ? mul8(y, load_param(cols, a, a.w1, 0, 0)) : y;
+      if (a.b1) u = add8(u, load_param(cols, a, a.b1, 0, 0));
     }
+    F8 d = expand(s_raw);
     if (n2) {                          // h becomes hhat, d the gradient of s
-#pragma unroll
-      for (int j = 0; j < 8; ++j) h[j] = fmaf(a.alpha, h[j], a.beta * (gate[j] * u[j]));
-      float (&h1)[1][8] = *reinterpret_cast<float (*)[1][8]>(&h);
-      const float2 st = row_stats<1>(team, cols, h1, a.out_norm == SOUFFLE_NORM_RMS, a.eps2);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        h[j] = cols.has(0, j) ? (h[j] - st.x) * st.y : 0.0f;
-        if (g.dvec[SUM_W2]) add(SUM_W2, j, e[j] * h[j]);
-        if (g.dvec[SUM_B2]) add(SUM_B2, j, e[j]);
-      }
-      if (a.w2) {
-        cols.load(static_cast<const P*>(a.w2), 0, w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] *= w[j];
-      }
-      float2 m = make_float2(0.0f, 0.0f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        m.x += e[j];
-        m.y = fmaf(e[j], h[j], m.y);
-      }
-      m = team.sum(m);
-      m.x = a.out_norm == SOUFFLE_NORM_RMS ? 0.0f : m.x * team.inv_cols;
-      m.y *= team.inv_cols;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) d[j] = fmaf(st.y, e[j] - m.x - h[j] * m.y, d[j]);
+      h = mul8(h, a.alpha);
+      h = a.gate ? fma8(u, mul8(gate, a.beta), h) : fma8(u, a.beta, h);
+      const float mean_w = rms2 ? 0.0f : warp_total(sum8(h)) * team.inv_warp_cols;
+      h = cols.mask(0, add8(h, -mean_w * in));
+      F8 e = expand(o_raw);
+      if (a.w2) e = mul8(e, load_param(cols, a, a.w2, 0, 0));
+      const float4 st = team.merge(mean_w, warp_total4(dot8(h, h), sum8(e), dot8(e, h), 0.0f, team.lane));
+      const float rstd = rsqrtf(st.y * team.inv_cols + a.eps2);
+      if (team.warps > 1 && !rms2) h = cols.mask(0, add8(h, (mean_w - st.x) * in));
+      h = mul8(h, rstd);
+      // d += rstd (e - mean e - hhat mean (e hhat))
+      e = fma8(h, -rstd * st.w * team.inv_cols, e);
+      if (!rms2) e = cols.mask(0, add8(e, -st.z * team.inv_cols * in));
+      d = fma8(e, rstd, d);
+      if (g.dvec[SUM_W2]) add(SUM_W2, expand(o_raw), h);
+      if (g.dvec[SUM_B2]) add1(SUM_B2, expand(o_raw));
     }
-    if (g.dr) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = a.alpha * d[j];
-      cols.store(static_cast<T*>(g.dr) + row * g.dr_stride, 0, w);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      d[j] *= a.beta;
-      if (g.dgate) add(SUM_GATE, j, d[j] * u[j]);
-      d[j] *= gate[j];
-    }
+    if (g.dr) cols.store(static_cast<T*>(g.dr) + row * g.dr_stride, 0, mul8(d, a.alpha));
+    if (g.dgate) add(SUM_GATE, d, u);  // beta comes in at the end
+    d = mul8(d, a.beta);
+    if (a.gate) d = mul8(d, gate);
     if (n1) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (g.dvec[SUM_W1]) add(SUM_W1, j, d[j] * y[j]);
-        if (g.dvec[SUM_B1]) add(SUM_B1, j, d[j]);
-      }
-      if (a.w1) {
-        cols.load(static_cast<const P*>(a.w1), 0, w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] *= w[j];
-      }
-      float2 m = make_float2(0.0f, 0.0f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (cols.has(0, j)) m.x += d[j];
-        m.y = fmaf(d[j], y[j], m.y);
-      }
-      m = team.sum(m);
-      m.x = a.branch_norm == SOUFFLE_NORM_RMS ? 0.0f : m.x * team.inv_cols;
-      m.y *= team.inv_cols;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) d[j] = rstd1 * (d[j] - m.x - y[j] * m.y);
+      if (g.dvec[SUM_W1]) add(SUM_W1, d, y);
+      if (g.dvec[SUM_B1]) add1(SUM_B1, d);
+      if (a.w1) d = mul8(d, load_param(cols, a, a.w1, 0, 0));
+      const float4 m = team.exchange(warp_total4(sum8(d), dot8(d, y), 0.0f, 0.0f, team.lane));
+      d = fma8(y, -m.y * team.inv_cols, d);
+      if (!rms1) d = add8(d, -m.x * team.inv_cols);
+      d = mul8(d, rstd1);
     }
     if (g.dy) cols.store(static_cast<T*>(g.dy) + row * g.dy_stride, 0, d);
-    if (g.dgate && a.gate_rows > 1 && ((row + 1) % per_gate == 0 || row + 1 == end)) {
-      const int first = row / per_gate * per_gate;
-      float v[8];
-      take(SUM_GATE, v, true);
-      if (first >= begin && first + per_gate <= end) cols.store(static_cast<P*>(g.dgate) + (long long)(row / per_gate) * a.cols, 0, v);
-      else cols.store(g.slots + (2LL * id + (first > begin)) * a.cols, 0, v);
+    const bool last_of_gate = row + 1 - gate_first == per_gate;
+    if (g.dgate && a.gate_rows > 1 && (last_of_gate || row + 1 == end)) {
+      const F8 v = mul8(take(SUM_GATE), a.beta);
+      if (gate_first >= begin && last_of_gate) store_param(cols, a, g.dgate, gate_at, v);
+      else cols.store(g.slots + (2LL * id + (gate_first > begin)) * a.cols, 0, v);
+    }
+    if (last_of_gate) {
+      ++gate_at;
+      gate_first += per_gate;
     }
   }
 
-  // the teams of the CTA, one sum at a time
+  // The teams of the CTA, one sum at a time: each team lays its columns down, every thread adds up some.
   const bool have[SUMS] = {g.dvec[SUM_W1] != nullptr, g.dvec[SUM_B1] != nullptr, g.dvec[SUM_W2] != nullptr, g.dvec[SUM_B2] != nullptr,
                            g.dgate && a.gate_rows == 1};
 #pragma unroll
   for (int k = 0; k < SUMS; ++k) {
     if (!have[k]) continue;
     float* part = g.part + ((long long)blockIdx.x * SUMS + k) * a.cols;
-    float v[8];
-    take(k, v, false);
+    const F8 v = k == SUM_GATE ? mul8(take(k), a.beta) : take(k);
     if (teams == 1) {
       cols.store(part, 0, v);
       continue;
     }
-    for (int t = 0; t < teams; ++t) {
-      __syncthreads();
-      if (t == mine) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (cols.has(0, j)) sums[cols.at(0, j)] = t == 0 ? v[j] : sums[cols.at(0, j)] + v[j];
-      }
-    }
     __syncthreads();
-    for (int c = threadIdx.x; c < a.cols; c += blockDim.x) part[c] = sums[c];
+    cols.store(sums + mine * a.cols, 0, v);
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
+      float total = sums[c];
+      for (int t = 1; t < teams; ++t) total += sums[t * a.cols + c];
+      part[c] = total;
+    }
   }
 }
 
-// Adds up what the CTAs left.  y < 4: a vector's sum; y = 4: the one gate row's; y = SUMS + t: that of the gate whose last rows are
-// team t's and whose first ones are not (any other gate was written by its one team).
-constexpr int kFinishLanes = 16;
+// The same with rows through the ring, eight columns a lane; widths up to 256 kGradWarps.
+constexpr int kGradRowWarps = 16;
+template <class T, bool kFull, bool kN1, bool kN2>
+__global__ void __launch_bounds__(32 * kGradRowWarps, 1) souffle_residual_norm_grad_rows(const NormGradArgs g, const RowPlan p) {
+  extern __shared__ __align__(128) char smem[];
+  const NormArgs& a = g.f;
+  RowCtl& ctl = *reinterpret_cast<RowCtl*>(smem);
+  const int warp = threadIdx.x >> 5, mine = warp / p.warps, t = threadIdx.x - mine * 32 * p.warps;
+  const int id = blockIdx.x * p.teams + mine, n = a.cols;
+  char* own = smem + 64 + mine * p.team_bytes;
+  const Columns<true> cols = {t, 32 * p.warps, n};
+  const int c = 8 * t, plane = plane_floats(n);
+  float* gate_s = reinterpret_cast<float*>(own + team_gate_at()) + plane_at(c);
+  const bool has = kFull || c < n;
+  float* vec = reinterpret_cast<float*>(smem + p.vectors);
+  const int begin = first_row(id, a.rows, g.teams), end = first_row(id + 1LL, a.rows, g.teams);
+  const bool have_r = a.r != nullptr, have_ds = g.ds != nullptr, have_gate = a.gate != nullptr;
+  RowRing<4> ring;                             // y, r, do, ds
+  ring.step[0] = a.y_stride * (long long)sizeof(T);
+  ring.step[1] = a.r_stride * (long long)sizeof(T);
+  ring.step[2] = g.do_stride * (long long)sizeof(T);
+  ring.step[3] = g.ds_stride * (long long)sizeof(T);
+  ring.from[0] = static_cast<const char*>(a.y) + begin * ring.step[0];
+  ring.from[1] = kN2 && have_r ? static_cast<const char*>(a.r) + begin * ring.step[1] : nullptr;
+  ring.from[2] = kN2 ? static_cast<const char*>(g.dout) + begin * ring.step[2] : nullptr;
+  ring.from[3] = have_ds ? static_cast<const char*>(g.ds) + begin * ring.step[3] : nullptr;
+  ring.at0 = own + team_ring_at(n, have_gate);
+  ring.bars = smem_u32(own + kTeamBox);
+  ring.parity = 0;
+  ring.slots = p.slots, ring.row_bytes = p.row_bytes, ring.operands = p.operands, ring.slot = 0;
+  ring.left = end - begin;
+  if (t == 0) ring.begin();
+  row_ctl_begin(ctl);
+  if (kN1 && kN2) lay_vectors<3>(vec, a, {a.w1, a.b1, a.w2});
+  else if (kN1) lay_vectors<2>(vec, a, {a.w1, a.b1});
+  else if (kN2) lay_vectors<1>(vec, a, {a.w2});
+  const float *w1 = vec + plane_at(c), *b1 = w1 + plane, *w2 = w1 + (kN1 ? 2 * plane : 0);
+  Team team;
+  team.begin(own, p.warps, warp - mine * p.warps, 1 + mine, cols, 1);
+  __syncthreads();
+
+  F8 acc[SUMS];
+#pragma unroll
+  for (int k = 0; k < SUMS; ++k) acc[k] = all8(0.0f);
+  const int per_gate = have_gate ? a.rows / a.gate_rows : 0x7fffffff;
+  int gate_at = have_gate ? begin / per_gate : 0, gate_first = gate_at * per_gate;       // the row's gate, and that one's first row
+  bool gate_new = have_gate;
+  const bool rms1 = a.branch_norm == SOUFFLE_NORM_RMS, rms2 = a.out_norm == SOUFFLE_NORM_RMS;
+  T *dr = static_cast<T*>(g.dr) + begin * g.dr_stride + c, *dy = static_cast<T*>(g.dy) + begin * g.dy_stride + c;
+  for (int row = begin; row < end; ++row) {
+    if (gate_new && has) write_plane(gate_s, mul8(read_param(a, a.gate, (long long)gate_at * n + c), a.beta));       // it is read by who wrote it
+    gate_new = false;
+    const char* slot = ring.wait(ctl.wait) + c * (int)sizeof(T);
+    F8 y = has ? expand(read16(reinterpret_cast<const T*>(slot))) : all8(0.0f), u = y;
+    float rstd1 = 1.0f;
+    if (kN1) {                         // y becomes yhat, u = N1(y)
+      const float mean_w = rms1 ? 0.0f : warp_total(sum8(y)) * team.inv_warp_cols;
+      if (!rms1) y = add8(y, has ? -mean_w : 0.0f);
+      float m2 = warp_total(dot8(y, y));
+      if (team.warps > 1) {
+        const float4 st = team.merge(mean_w, m2);
+        m2 = st.y;
+        if (!rms1) y = add8(y, has ? mean_w - st.x : 0.0f);
+      }
+      rstd1 = rsqrtf(m2 * team.inv_cols + a.eps1);
+      y = mul8(y, rstd1);
+      if (has) u = fma8(y, read_plane(w1), read_plane(b1));
+    }
+    F8 d = all8(0.0f);
+    if (kN2) {                         // h becomes hhat, d the gradient of s
+      F8 h = have_gate ? (has ? mul8(u, read_plane(gate_s)) : u) : mul8(u, a.beta), e = d, o = d;
+      const char* at = slot + ring.row_bytes;
+      if (has) {
+        if (have_r) {
+          h = fma8(expand(read16(reinterpret_cast<const T*>(at))), a.alpha, h);
+          at += ring.row_bytes;
+        }
+        o = expand(read16(reinterpret_cast<const T*>(at)));
+        if (have_ds) d = expand(read16(reinterpret_cast<const T*>(at + ring.row_bytes)));
+        e = mul8(o, read_plane(w2));
+      }
+      const float mean_w = rms2 ? 0.0f : warp_total(sum8(h)) * team.inv_warp_cols;
+      if (!rms2) h = add8(h, has ? -mean_w : 0.0f);
+      const float4 st = team.merge(mean_w, warp_total4(dot8(h, h), sum8(e), dot8(e, h), 0.0f, team.lane));
+      const float rstd = rsqrtf(st.y * team.inv_cols + a.eps2);
+      if (!rms2 && team.warps > 1) h = add8(h, has ? mean_w - st.x : 0.0f);
+      h = mul8(h, rstd);
+      acc[SUM_W2] = fma8(o, h, acc[SUM_W2]);
+      acc[SUM_B2] = add8(acc[SUM_B2], o);
+      // d += rstd (e - mean e - hhat mean (e hhat))
+      e = fma8(h, -rstd * st.w * team.inv_cols, e);
+      if (!rms2) e = add8(e, has ? -st.z * team.inv_cols : 0.0f);
+      d = fma8(e, rstd, d);
+    } else if (have_ds && has) {
+      d = expand(read16(reinterpret_cast<const T*>(slot + ring.row_bytes)));
+    }
+    if (g.dr && has) write16(dr, narrow<T>(mul8(d, a.alpha)));
+    if (g.dgate) acc[SUM_GATE] = fma8(d, u, acc[SUM_GATE]);         // beta comes in at the end
+    if (have_gate) {
+      if (has) d = mul8(d, read_plane(gate_s));
+    } else {
+      d = mul8(d, a.beta);
+    }
+    if (kN1) {
+      acc[SUM_W1] = fma8(d, y, acc[SUM_W1]);
+      acc[SUM_B1] = add8(acc[SUM_B1], d);
+      if (has) d = mul8(d, read_plane(w1));
+      const float4 m = team.exchange(warp_total4(sum8(d), dot8(d, y), 0.0f, 0.0f, team.lane));
+      d = fma8(y, -m.y * team.inv_cols, d);
+      if (!rms1) d = add8(d, -m.x * team.inv_cols);
+      d = mul8(d, rstd1);
+    }
+    if (team.warps == 1) __syncwarp();
+    else if (!kN1) team.meet();        // (behind the exchange everybody has read the slot)
+    ring.release(t == 0);
+    if (g.dy && has) write16(dy, narrow<T>(d));
+    dr += g.dr_stride;
+    dy += g.dy_stride;
+    const bool last_of_gate = row + 1 - gate_first == per_gate;
+    if (g.dgate && a.gate_rows > 1 && (last_of_gate || row + 1 == end)) {
+      const F8 v = mul8(acc[SUM_GATE], a.beta);
+      acc[SUM_GATE] = all8(0.0f);
+      if (gate_first >= begin && last_of_gate) store_param(cols, a, g.dgate, gate_at, v);
+      else cols.store(g.slots + (2LL * id + (gate_first > begin)) * n, 0, v);
+    }
+    if (last_of_gate) {
+      ++gate_at;
+      gate_first += per_gate;
+      gate_new = have_gate;
+    }
+  }
+
+  // the teams of the CTA, one sum at a time, in what was the rings and vectors
+  float* sums = reinterpret_cast<float*>(smem + 64);
+#pragma unroll
+  for (int k = 0; k < SUMS; ++k) {
+    const bool want = k < SUM_GATE ? g.dvec[k] != nullptr : g.dgate && a.gate_rows == 1;
+    if (!want) continue;
+    float* part = g.part + ((long long)blockIdx.x * SUMS + k) * n;
+    const F8 v = k == SUM_GATE ? mul8(acc[k], a.beta) : acc[k];
+    if (p.teams == 1) {
+      cols.store(part, 0, v);
+      continue;
+    }
+    __syncthreads();
+    if (has) write_plane(sums + mine * plane + plane_at(c), v);
+    __syncthreads();
+    for (int i = threadIdx.x; i < n >> 3; i += blockDim.x) {
+      const float* at = sums + plane_at(8 * i);
+      F8 total = read_plane(at);
+      for (int k2 = 1; k2 < p.teams; ++k2) total = add8(total, read_plane(at + k2 * plane));
+      write16(part + 8 * i, narrow<float>(total));
+    }
+  }
+  row_ctl_end(ctl);
+}
+
+// Adds up what the CTAs left.  y < 4: a vector's sum; y = 4: the one gate row's; y >= SUMS: that of a gate whose rows several teams
+// shared (any other gate was written by its one team): gate y - SUMS, or, where there are more gates than teams, the gate whose
+// last rows are team y - SUMS's.
+constexpr int kFinishLanes = 8;
 template <class P>
 __global__ void __launch_bounds__(32 * kFinishLanes) souffle_residual_norm_grad_sums(const NormGradArgs g, int ctas) {
   __shared__ float sm[kFinishLanes][33];
@@ -320,14 +667,22 @@ __global__ void __launch_bounds__(32 * kFinishLanes) souffle_residual_norm_grad_
     to = static_cast<P*>(k < SUM_GATE ? g.dvec[k] : a.gate_rows == 1 ? g.dgate : nullptr);
     if (!to) return;
     if (c < a.cols)
+#pragma unroll 8
       for (int i = lane; i < ctas; i += kFinishLanes) v += g.part[((long long)i * SUMS + k) * a.cols + c];
   } else {
-    const int t1 = k - SUMS, per_gate = a.rows / a.gate_rows, begin = first_row(t1, a.rows, g.teams), end = first_row(t1 + 1LL, a.rows, g.teams);
-    const int first = begin / per_gate * per_gate;
-    if (first == begin || begin == end || first + per_gate > end) return;
-    const int t0 = (int)(((first + 1LL) * g.teams - 1) / a.rows);       // the team of row `first`
-    to = static_cast<P*>(g.dgate) + (long long)(begin / per_gate) * a.cols;
+    const int per_gate = a.rows / a.gate_rows;
+    int gate = k - SUMS;
+    if (a.gate_rows > g.teams) {
+      const int begin = first_row(k - SUMS, a.rows, g.teams), end = first_row(k - SUMS + 1LL, a.rows, g.teams);
+      gate = begin / per_gate;
+      if (begin == end || gate * per_gate == begin || (gate + 1) * per_gate > end) return;
+    }
+    const int first = gate * per_gate, last = first + per_gate - 1;
+    const int t0 = (int)(((first + 1LL) * g.teams - 1) / a.rows), t1 = (int)(((last + 1LL) * g.teams - 1) / a.rows);     // their teams
+    if (t0 == t1) return;
+    to = static_cast<P*>(g.dgate) + (long long)gate * a.cols;
     if (c < a.cols)
+#pragma unroll 2
       for (int t = t0 + lane; t <= t1; t += kFinishLanes) {
         const int from = first_row(t, a.rows, g.teams);
         if (from < first_row(t + 1LL, a.rows, g.teams)) v += g.slots[(2LL * t + (first > from)) * a.cols + c];
@@ -342,15 +697,15 @@ __global__ void __launch_bounds__(32 * kFinishLanes) souffle_residual_norm_grad_
 
 // ---- host --------------------------------------------------------------------------------------------------------
 
-constexpr int kMaxNormCols = 8192;
+constexpr int kMaxNormCols = 8192, kMaxNormRows = 1 << 30;
 
 static size_t dtype_size(int t) { return t == SOUFFLE_F32 ? 4 : 2; }
 // whether rows of `stride` elements from `p` on can be read 16 bytes at a time
 static bool wide_rows(const void* p, long long stride, size_t size) { return !p || (((uintptr_t)p | (uintptr_t)(stride * (long long)size)) & 15u) == 0; }
 
 static int check_norm(const SouffleResidualNorm& d, bool forward, bool* vec) {
-  if (d.rows < 0 || d.cols < 1 || d.cols > kMaxNormCols)
-    return fail(SOUFFLE_BAD_SHAPE, "residual norm of %d x %d: rows >= 0 and 1 <= cols <= %d are wanted", d.rows, d.cols, kMaxNormCols);
+  if (d.rows < 0 || d.rows > kMaxNormRows || d.cols < 1 || d.cols > kMaxNormCols)
+    return fail(SOUFFLE_BAD_SHAPE, "residual norm of %d x %d: 0 <= rows <= %d and 1 <= cols <= %d are wanted", d.rows, d.cols, kMaxNormRows, kMaxNormCols);
   if (d.dtype < SOUFFLE_F32 || d.dtype > SOUFFLE_BF16 || (d.param_dtype != d.dtype && d.param_dtype != SOUFFLE_F32))
     return fail(SOUFFLE_BAD_ARGUMENT, "dtype %d with param_dtype %d: values are fp32, fp16 or bf16, vectors the same or fp32", d.dtype, d.param_dtype);
   for (int n : {d.branch_norm, d.out_norm})
@@ -392,24 +747,90 @@ static NormArgs norm_args(const SouffleResidualNorm& d) {
   a.r_stride = d.residual_stride; a.y_stride = d.branch_stride; a.s_stride = d.sum_stride; a.o_stride = d.out_stride; a.q_stride = d.out_q_stride;
   a.r = d.residual; a.y = d.branch; a.gate = d.gate;
   a.w1 = d.branch_weight; a.b1 = d.branch_bias; a.w2 = d.out_weight; a.b2 = d.out_bias;
+  a.param_dtype = d.param_dtype;
   a.s = d.sum; a.o = d.out; a.q = static_cast<signed char*>(d.out_q); a.q_scale = d.out_scale;
   return a;
 }
 
-template <class T, class P, bool kVec>
-static int forward_groups(const NormArgs& a, cudaStream_t st) {
-  const int groups8 = (a.cols + 7) / 8;
-  // A warp per row up to 1024 columns, several beyond that, four groups of eight columns a thread.
-  const int warps = groups8 <= 128 ? 1 : (groups8 + 127) / 128;
-  const int groups = (groups8 + 32 * warps - 1) / (32 * warps);
-  const int threads = warps == 1 ? 128 : 32 * warps, teams = threads / (32 * warps);
-  const int grid = (a.rows + teams - 1) / teams;
-  switch (groups) {
-    case 1: souffle_residual_norm<T, P, kVec, 1><<<grid, threads, 0, st>>>(a, warps); break;
-    case 2: souffle_residual_norm<T, P, kVec, 2><<<grid, threads, 0, st>>>(a, warps); break;
-    case 3: souffle_residual_norm<T, P, kVec, 3><<<grid, threads, 0, st>>>(a, warps); break;
-    default: souffle_residual_norm<T, P, kVec, 4><<<grid, threads, 0, st>>>(a, warps); break;
+constexpr int kRowWarps = 24, kRowSmem = 220 * 1024;
+
+// How rows go through the ring: `groups` groups of eight columns a thread at most, operands of a row, vectors.  False: they do not fit.
+static bool row_plan(int rows, int cols, int elem, int operands, bool gate, int vectors, int max_groups, int max_warps, int sms, RowPlan* p, int* groups,
+                     int* grid, int* smem) {
+  const int groups8 = cols / 8;
+  p->warps = (groups8 + 32 * max_groups - 1) / (32 * max_groups);
+  if (p->warps > max_warps) return false;
+  *groups = (groups8 + 32 * p->warps - 1) / (32 * p->warps);
+  p->row_bytes = cols * elem;
+  p->operands = operands;
+  const int fit = max_warps / p->warps, most = p->warps > 1 && fit > 15 ? 15 : fit;      // teams of several warps have named barriers 1 .. 15
+  const int want = (rows + sms - 1) / sms;
+  p->teams = want < most ? want : most;
+  const int vector_bytes = vectors * plane_floats(cols) * 4;
+  for (;; --p->teams) {
+    if (p->teams < 1) return false;
+    const int fixed = (team_ring_at(cols, gate) + 127) / 128 * 128, room = (kRowSmem - 64 - 128 - vector_bytes) / p->teams - fixed - 128;
+    p->slots = room / (operands * p->row_bytes);
+    const int per_team = (rows + p->teams * sms - 1) / (p->teams * sms);
+    if (p->slots > kMaxRowSlots) p->slots = kMaxRowSlots;
+    if (p->slots > per_team) p->slots = per_team;
+    if (p->slots >= 2 || (p->slots == 1 && (per_team == 1 || p->teams == 1))) {
+      p->team_bytes = (team_ring_at(cols, gate) + p->slots * operands * p->row_bytes + 127) / 128 * 128;
+      break;
+    }
   }
+  const int need = (rows + p->teams - 1) / p->teams;
+  *grid = need < sms ? need : sms;
+  p->total_teams = *grid * p->teams;
+  p->vectors = 64 + p->teams * p->team_bytes;
+  *smem = p->vectors + vector_bytes;
+  return true;
+}
+
+// Launches one of these kernels, whose shared memory the first call of each on a device has to allow.
+template <class F, class A> static int launch_rows(F fn, const A& a, const RowPlan& p, int grid, int smem, int dev, bool (&ready)[kMaxDevices], cudaStream_t st) {
+  if (!ready[dev]) {
+    SF_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSmem));
+    ready[dev] = true;
+  }
+  fn<<<grid, 32 * p.warps * p.teams, smem, st>>>(a, p);
+  SF_CUDA(cudaGetLastError());
+  return SOUFFLE_OK;
+}
+template <class T, bool kFull, int kGroups, bool kN1>
+static int forward_rows(const NormArgs& a, const RowPlan& p, int grid, int smem, int dev, cudaStream_t st) {
+  static bool ready[kMaxDevices];
+  return launch_rows(souffle_residual_norm_rows<T, kFull, kGroups, kN1>, a, p, grid, smem, dev, ready, st);
+}
+template <class T, bool kFull, bool kN1>
+static int forward_rows(const NormArgs& a, const RowPlan& p, int groups, int grid, int smem, int dev, cudaStream_t st) {
+  switch (groups) {
+    case 1: return forward_rows<T, kFull, 1, kN1>(a, p, grid, smem, dev, st);
+    case 2: return forward_rows<T, kFull, 2, kN1>(a, p, grid, smem, dev, st);
+    case 3: return forward_rows<T, kFull, 3, kN1>(a, p, grid, smem, dev, st);
+    default: return forward_rows<T, kFull, 4, kN1>(a, p, grid, smem, dev, st);
+  }
+}
+
+template <class T>
+static int forward_launch(const NormArgs& a, bool vec, int sms, int dev, cudaStream_t st) {
+  RowPlan p;
+  int groups, grid, smem;
+  const bool n1 = a.branch_norm != SOUFFLE_NORM_NONE;
+  // Few rows: as many warps on a row as there are; many: as few as hold it
+  int max_groups = a.rows <= sms ? (a.cols + 256 * kRowWarps - 1) / (256 * kRowWarps) : 4;
+  if (vec && row_plan(a.rows, a.cols, sizeof(T), a.r ? 2 : 1, a.gate, n1 ? 4 : 2, max_groups, kRowWarps, sms, &p, &groups, &grid, &smem)) {
+    const bool full = a.cols == 256 * p.warps * groups;
+    if (n1) return full ? forward_rows<T, true, true>(a, p, groups, grid, smem, dev, st) : forward_rows<T, false, true>(a, p, groups, grid, smem, dev, st);
+    return full ? forward_rows<T, true, false>(a, p, groups, grid, smem, dev, st) : forward_rows<T, false, false>(a, p, groups, grid, smem, dev, st);
+  }
+  const int groups8 = (a.cols + 7) / 8, warps = groups8 <= 128 ? 1 : (groups8 + 127) / 128;
+  groups = (groups8 + 32 * warps - 1) / (32 * warps);
+  const int threads = warps == 1 ? 128 : 32 * warps, teams = threads / (32 * warps);
+  grid = (a.rows + teams - 1) / teams;
+  if (groups == 1) souffle_residual_norm_any<T, 1><<<grid, threads, 0, st>>>(a, warps);
+  else if (groups == 2) souffle_residual_norm_any<T, 2><<<grid, threads, 0, st>>>(a, warps);
+  else souffle_residual_norm_any<T, 4><<<grid, threads, 0, st>>>(a, warps);
   SF_CUDA(cudaGetLastError());
   return SOUFFLE_OK;
 }
@@ -419,35 +840,77 @@ struct GradGrid { int warps, per_cta, ctas; };
 static GradGrid grad_grid(int rows, int cols, int sms) {
   GradGrid g;
   g.warps = (cols + 255) / 256;
-  g.per_cta = g.warps > 16 ? 1 : 16 / g.warps > 15 ? 15 : 16 / g.warps;       // named barriers 1 .. 15
+  g.per_cta = g.warps > kGradWarps ? 1 : kGradWarps / g.warps > 15 ? 15 : kGradWarps / g.warps;       // named barriers 1 .. 15
   const int need = (rows + g.per_cta - 1) / g.per_cta;
   g.ctas = need < sms ? need : sms;
   return g;
 }
 
-template <class T, class P, bool kVec, bool kSharedSums>
-static int backward_launch(NormGradArgs& g, const GradGrid& gg, cudaStream_t st) {
-  auto fn = souffle_residual_norm_grad<T, P, kVec, kSharedSums>;
-  const int threads = 32 * gg.warps * gg.per_cta;
-  const int smem = gg.per_cta * kTeamBox + (kSharedSums ? SUMS * 8 * threads : gg.per_cta > 1 ? g.f.cols : 0) * (int)sizeof(float);
-  if (smem > 48 * 1024) SF_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  fn<<<gg.ctas, threads, smem, st>>>(g, gg.warps);
-  SF_CUDA(cudaGetLastError());
-  const bool gates = g.dgate && g.f.gate_rows > 1;
-  bool any = g.dgate;
+// The sums over CTAs and teams, behind either kernel.
+static int finish_sums(const NormGradArgs& g, int ctas, cudaStream_t st) {
+  const int shared_gates = !g.dgate || g.f.gate_rows <= 1 || g.f.gate_rows == g.f.rows ? 0 : g.f.gate_rows < g.teams ? g.f.gate_rows : g.teams;
+  bool any = g.dgate && (g.f.gate_rows == 1 || shared_gates);
   for (void* p : g.dvec) any = any || p;
-  if (any) {
-    souffle_residual_norm_grad_sums<P><<<dim3((g.f.cols + 31) / 32, SUMS + (gates ? g.teams : 0)), 32 * kFinishLanes, 0, st>>>(g, gg.ctas);
-    SF_CUDA(cudaGetLastError());
-  }
+  if (!any) return SOUFFLE_OK;
+  const dim3 grid((g.f.cols + 31) / 32, SUMS + shared_gates);
+  if (g.f.param_dtype == SOUFFLE_F32) souffle_residual_norm_grad_sums<float><<<grid, 32 * kFinishLanes, 0, st>>>(g, ctas);
+  else if (g.f.param_dtype == SOUFFLE_F16) souffle_residual_norm_grad_sums<__half><<<grid, 32 * kFinishLanes, 0, st>>>(g, ctas);
+  else souffle_residual_norm_grad_sums<__nv_bfloat16><<<grid, 32 * kFinishLanes, 0, st>>>(g, ctas);
+  SF_CUDA(cudaGetLastError());
   return SOUFFLE_OK;
 }
 
-// Calls f with the types of (dtype, param_dtype) as arguments' types.
-template <class F> static int with_types(int dtype, int param_dtype, F f) {
-  if (dtype == SOUFFLE_F32) return f(0.0f, 0.0f);
-  if (dtype == SOUFFLE_F16) return param_dtype == SOUFFLE_F32 ? f(__half(), 0.0f) : f(__half(), __half());
-  return param_dtype == SOUFFLE_F32 ? f(__nv_bfloat16(), 0.0f) : f(__nv_bfloat16(), __nv_bfloat16());
+template <class T, bool kVec, bool kSharedSums>
+static int backward_any(const NormGradArgs& g, const GradGrid& gg, cudaStream_t st) {
+  auto fn = souffle_residual_norm_grad<T, kVec, kSharedSums>;
+  const int threads = 32 * gg.warps * gg.per_cta;
+  const int smem = gg.per_cta * kTeamBox + (kSharedSums ? SUMS * 8 * threads : gg.per_cta > 1 ? gg.per_cta * ((g.f.cols + 3) & ~3) : 0) * (int)sizeof(float);
+  if (smem > 48 * 1024) SF_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  fn<<<gg.ctas, threads, smem, st>>>(g, gg.warps);
+  SF_CUDA(cudaGetLastError());
+  return SOUFFLE_OK;
+}
+template <class T, bool kFull, bool kN1, bool kN2>
+static int backward_rows(const NormGradArgs& g, const RowPlan& p, int grid, int smem, int dev, cudaStream_t st) {
+  static bool ready[kMaxDevices];
+  return launch_rows(souffle_residual_norm_grad_rows<T, kFull, kN1, kN2>, g, p, grid, smem, dev, ready, st);
+}
+template <class T, bool kFull>
+static int backward_rows(const NormGradArgs& g, const RowPlan& p, int grid, int smem, int dev, cudaStream_t st) {
+  const bool n1 = g.f.branch_norm != SOUFFLE_NORM_NONE, n2 = g.f.out_norm != SOUFFLE_NORM_NONE;
+  if (n1) return n2 ? backward_rows<T, kFull, true, true>(g, p, grid, smem, dev, st) : backward_rows<T, kFull, true, false>(g, p, grid, smem, dev, st);
+  return n2 ? backward_rows<T, kFull, false, true>(g, p, grid, smem, dev, st) : backward_rows<T, kFull, false, false>(g, p, grid, smem, dev, st);
+}
+
+// `g` without the workspace's layout, which depends on the grid.
+template <class T>
+static int backward_launch(NormGradArgs& g, bool vec, float* workspace, int sms, int dev, cudaStream_t st) {
+  RowPlan p;
+  int groups, grid, smem, ctas, rc;
+  const bool n1 = g.f.branch_norm != SOUFFLE_NORM_NONE, n2 = g.f.out_norm != SOUFFLE_NORM_NONE;
+  g.part = workspace;
+  if (vec && row_plan(g.f.rows, g.f.cols, sizeof(T), 1 + (n2 && g.f.r) + n2 + (g.ds != nullptr), g.f.gate, 2 * n1 + n2, 1, kGradRowWarps, sms, &p, &groups,
+                      &grid, &smem)) {
+    // behind the rows the teams' sums lie in the rings' place
+    if (p.teams > 1 && smem < 64 + p.teams * plane_floats(g.f.cols) * 4) smem = 64 + p.teams * plane_floats(g.f.cols) * 4;
+    ctas = grid;
+    g.teams = p.total_teams;
+    g.slots = g.part + (size_t)ctas * SUMS * g.f.cols;
+    rc = g.f.cols == 256 * p.warps ? backward_rows<T, true>(g, p, grid, smem, dev, st) : backward_rows<T, false>(g, p, grid, smem, dev, st);
+  } else {
+    const GradGrid gg = grad_grid(g.f.rows, g.f.cols, sms);
+    ctas = gg.ctas;
+    g.teams = gg.ctas * gg.per_cta;
+    g.slots = g.part + (size_t)ctas * SUMS * g.f.cols;
+    if (gg.warps > kGradWarps) rc = vec ? backward_any<T, true, true>(g, gg, st) : backward_any<T, false, true>(g, gg, st);
+    else rc = vec ? backward_any<T, true, false>(g, gg, st) : backward_any<T, false, false>(g, gg, st);
+  }
+  return rc ? rc : finish_sums(g, ctas, st);
+}
+
+// Calls f with a value of the type of `dtype`.
+template <class F> static int with_type(int dtype, F f) {
+  return dtype == SOUFFLE_F32 ? f(0.0f) : dtype == SOUFFLE_F16 ? f(__half()) : f(__nv_bfloat16());
 }
 
 }  // namespace souffle
@@ -459,30 +922,27 @@ extern "C" {
 int souffle_residual_norm_forward(const SouffleResidualNorm* call, souffle_stream_t stream) {
   if (!call) return fail(SOUFFLE_BAD_ARGUMENT, "null call record");
   bool vec = false;
-  int rc = check_norm(*call, true, &vec), sms;
+  int rc = check_norm(*call, true, &vec), sms, dev;
   if (rc || call->rows == 0) return rc;
-  if ((rc = current_sms(&sms))) return rc;
+  if ((rc = current_sms(&sms, &dev))) return rc;
   const NormArgs a = norm_args(*call);
-  return with_types(call->dtype, call->param_dtype, [&](auto t, auto p) {
-    using T = decltype(t);
-    using P = decltype(p);
-    return vec ? forward_groups<T, P, true>(a, (cudaStream_t)stream) : forward_groups<T, P, false>(a, (cudaStream_t)stream);
-  });
+  return with_type(call->dtype, [&](auto t) { return forward_launch<decltype(t)>(a, vec, sms, dev, (cudaStream_t)stream); });
 }
 
-// The largest grid that any device of this library's kind gives: it has at most 160 SMs.
+// Enough for either kernel's grid: no more CTAs than SMs, of which a device of this library's kind has fewer than kMostSms, and
+// no more teams than 16 warps.
 static constexpr int kMostSms = 160;
 size_t souffle_residual_norm_backward_workspace_bytes(int32_t rows, int32_t cols, int32_t gate_rows) {
   if (rows < 1 || cols < 1 || cols > kMaxNormCols) return 0;
-  const GradGrid g = grad_grid(rows, cols, kMostSms);
-  return ((size_t)g.ctas * SUMS + (gate_rows > 1 ? 2 * (size_t)g.ctas * g.per_cta : 0)) * cols * sizeof(float);
+  const int warps = (cols + 255) / 256, per_cta = warps > 16 ? 1 : 16 / warps, ctas = rows < kMostSms ? rows : kMostSms;
+  return ((size_t)ctas * SUMS + (gate_rows > 1 ? 2 * (size_t)ctas * per_cta : 0)) * cols * sizeof(float);
 }
 
 int souffle_residual_norm_backward(const SouffleResidualNormGrad* call, souffle_stream_t stream) {
   if (!call) return fail(SOUFFLE_BAD_ARGUMENT, "null call record");
   const SouffleResidualNorm& d = call->f;
   bool vec = false;
-  int rc = check_norm(d, false, &vec), sms = 0;
+  int rc = check_norm(d, false, &vec), sms = 0, dev = 0;
   if (rc) return rc;
   const bool n2 = d.out_norm != SOUFFLE_NORM_NONE;
   if (d.rows > 0 && n2 != (call->grad_out != nullptr)) return fail(SOUFFLE_BAD_POINTER, "grad_out comes with a norm of the sum");
@@ -510,8 +970,8 @@ int souffle_residual_norm_backward(const SouffleResidualNormGrad* call, souffle_
   }
   if (!aligned16(call->workspace) || call->workspace_bytes < souffle_residual_norm_backward_workspace_bytes(d.rows, d.cols, d.gate_rows))
     return fail(SOUFFLE_BAD_POINTER, "workspace is null, misaligned or smaller than souffle_residual_norm_backward_workspace_bytes()");
-  if ((rc = current_sms(&sms))) return rc;
-  const GradGrid gg = grad_grid(d.rows, d.cols, sms < kMostSms ? sms : kMostSms);
+  if ((rc = current_sms(&sms, &dev))) return rc;
+  if (sms > kMostSms) sms = kMostSms;
   NormGradArgs g;
   memset(&g, 0, sizeof(g));
   g.f = norm_args(d);
@@ -519,16 +979,18 @@ int souffle_residual_norm_backward(const SouffleResidualNormGrad* call, souffle_
   g.ds = call->grad_sum; g.dout = call->grad_out;
   g.dr = call->d_residual; g.dy = call->d_branch; g.dgate = call->d_gate;
   g.dvec[SUM_W1] = call->d_branch_weight; g.dvec[SUM_B1] = call->d_branch_bias; g.dvec[SUM_W2] = call->d_out_weight; g.dvec[SUM_B2] = call->d_out_bias;
-  g.part = static_cast<float*>(call->workspace);
-  g.slots = g.part + (size_t)gg.ctas * SUMS * d.cols;
-  g.teams = gg.ctas * gg.per_cta;
-  return with_types(d.dtype, d.param_dtype, [&](auto t, auto p) {
-    using T = decltype(t);
-    using P = decltype(p);
-    cudaStream_t st = (cudaStream_t)stream;
-    if (gg.warps > 16) return vec ? backward_launch<T, P, true, true>(g, gg, st) : backward_launch<T, P, false, true>(g, gg, st);
-    return vec ? backward_launch<T, P, true, false>(g, gg, st) : backward_launch<T, P, false, false>(g, gg, st);
-  });
+  float* ws = static_cast<float*>(call->workspace);
+  return with_type(d.dtype, [&](auto t) { return backward_launch<decltype(t)>(g, vec, ws, sms, dev, (cudaStream_t)stream); });
+}
+
+int souffle_residual_norm_status(souffle_stream_t stream) {
+  SF_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
+  int h[4];
+  SF_CUDA(cudaMemcpyFromSymbol(h, g_norm_status, sizeof(h)));
+  if (h[0] == 0) return SOUFFLE_OK;
+  const int clear[4] = {0, 0, 0, 0};
+  SF_CUDA(cudaMemcpyToSymbol(g_norm_status, clear, sizeof(clear)));
+  return fail(SOUFFLE_DEVICE_TIMEOUT, "residual norm: device wait expired (code %d, where %d, cta %d)", h[0], h[1], h[2]);
 }
 
 }  // extern "C"

@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <string.h>
 
 namespace souffle {
 
@@ -16,48 +17,184 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Eight neighbouring values, from and to 16-byte aligned memory.
-template <class T> struct alignas(16) Eight { T v[8]; };
-template <class T> __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-  const Eight<T> e = *reinterpret_cast<const Eight<T>*>(p);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = to_f32(e.v[j]);
+// Eight neighbouring values as they are stored, moved 16 bytes at a time and converted in pairs.
+template <class T> struct alignas(16) Eight { uint32_t w[2 * sizeof(T)]; };
+
+// Eight columns in fp32 as four register pairs: the operations below are of both halves of a pair in one issue slot.
+struct F8 { uint64_t p[4]; };
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+  return p;
 }
-template <class T> __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+__device__ __forceinline__ float2 halves(uint64_t p) {
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ F8 all8(float v) {
+  const uint64_t p = pair(v, v);
+  return {{p, p, p, p}};
+}
+__device__ __forceinline__ F8 fma8(const F8& a, const F8& b, const F8& c) {
+  F8 d;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) d.p[i] = fma2(a.p[i], b.p[i], c.p[i]);
+  return d;
+}
+__device__ __forceinline__ F8 mul8(const F8& a, const F8& b) {
+  F8 d;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) d.p[i] = mul2(a.p[i], b.p[i]);
+  return d;
+}
+__device__ __forceinline__ F8 add8(const F8& a, const F8& b) {
+  F8 d;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) d.p[i] = add2(a.p[i], b.p[i]);
+  return d;
+}
+__device__ __forceinline__ F8 fma8(const F8& a, float b, const F8& c) { return fma8(a, all8(b), c); }
+__device__ __forceinline__ F8 mul8(const F8& a, float b) { return mul8(a, all8(b)); }
+__device__ __forceinline__ F8 add8(const F8& a, float b) { return add8(a, all8(b)); }
+__device__ __forceinline__ float sum8(const F8& a) {
+  const float2 v = halves(add2(add2(a.p[0], a.p[1]), add2(a.p[2], a.p[3])));
+  return v.x + v.y;
+}
+__device__ __forceinline__ float dot8(const F8& a, const F8& b) {
+  const float2 v = halves(add2(fma2(a.p[0], b.p[0], mul2(a.p[1], b.p[1])), fma2(a.p[2], b.p[2], mul2(a.p[3], b.p[3]))));
+  return v.x + v.y;
+}
+__device__ __forceinline__ void unpack8(const F8& a, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 h = halves(a.p[i]);
+    v[2 * i] = h.x;
+    v[2 * i + 1] = h.y;
+  }
+}
+__device__ __forceinline__ F8 pack8(const float (&v)[8]) { return {{pair(v[0], v[1]), pair(v[2], v[3]), pair(v[4], v[5]), pair(v[6], v[7])}}; }
+
+__device__ __forceinline__ uint64_t pair_of(const Eight<float>& e, int i) { return pair(__uint_as_float(e.w[2 * i]), __uint_as_float(e.w[2 * i + 1])); }
+__device__ __forceinline__ uint64_t pair_of(const Eight<__half>& e, int i) {
+  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&e.w[i]));
+  return pair(v.x, v.y);
+}
+__device__ __forceinline__ uint64_t pair_of(const Eight<__nv_bfloat16>& e, int i) {
+  return pair(__uint_as_float(e.w[i] << 16), __uint_as_float(e.w[i] & 0xffff0000u));
+}
+template <class T> __device__ __forceinline__ F8 expand(const Eight<T>& e) {
+  return {{pair_of(e, 0), pair_of(e, 1), pair_of(e, 2), pair_of(e, 3)}};
+}
+__device__ __forceinline__ void put_pair(Eight<float>& e, int i, float2 v) {
+  e.w[2 * i] = __float_as_uint(v.x);
+  e.w[2 * i + 1] = __float_as_uint(v.y);
+}
+__device__ __forceinline__ void put_pair(Eight<__half>& e, int i, float2 v) {
+  const __half2 h = __float22half2_rn(v);
+  e.w[i] = *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void put_pair(Eight<__nv_bfloat16>& e, int i, float2 v) {
+  const __nv_bfloat162 h = __float22bfloat162_rn(v);
+  e.w[i] = *reinterpret_cast<const uint32_t*>(&h);
+}
+template <class T> __device__ __forceinline__ Eight<T> narrow(const F8& a) {
   Eight<T> e;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) e.v[j] = from_f32<T>(v[j]);
-  *reinterpret_cast<Eight<T>*>(p) = e;
+  for (int i = 0; i < 4; ++i) put_pair(e, i, halves(a.p[i]));
+  return e;
+}
+// one of the eight
+template <class T> __device__ __forceinline__ T value_of(const Eight<T>& e, int j) {
+  T v;
+  if (sizeof(T) == 4) {
+    memcpy(&v, &e.w[j], 4);
+  } else {
+    const uint16_t bits = (uint16_t)(e.w[j >> 1] >> (16 * (j & 1)));
+    memcpy(&v, &bits, 2);
+  }
+  return v;
+}
+template <class T> __device__ __forceinline__ void put_value(Eight<T>& e, int j, const T* p) {      // into zeros
+  if (sizeof(T) == 4) e.w[j] = *reinterpret_cast<const uint32_t*>(p);
+  else e.w[j >> 1] |= (uint32_t)*reinterpret_cast<const uint16_t*>(p) << (16 * (j & 1));
+}
+template <class T> __device__ __forceinline__ Eight<T> zeros() {
+  Eight<T> e;
+#pragma unroll
+  for (int i = 0; i < (int)(2 * sizeof(T)); ++i) e.w[i] = 0u;
+  return e;
+}
+template <class T> __device__ __forceinline__ Eight<T> read16(const T* p) {
+  Eight<T> e;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+    const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+    e.w[4 * i] = v.x, e.w[4 * i + 1] = v.y, e.w[4 * i + 2] = v.z, e.w[4 * i + 3] = v.w;
+  }
+  return e;
+}
+template <class T> __device__ __forceinline__ void write16(T* p, const Eight<T>& e) {
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+    reinterpret_cast<uint4*>(p)[i] = make_uint4(e.w[4 * i], e.w[4 * i + 1], e.w[4 * i + 2], e.w[4 * i + 3]);
 }
 
 // The columns that thread `t` of a team of `team` threads holds: with kVec, group i is the eight columns from 8 (t + i team) on; without,
 // its eight columns are `team` apart, so that a team reads neighbouring elements whatever the alignment.
-template <bool kVec> struct Columns {
+template <bool kVec_> struct Columns {
+  static constexpr bool kVec = kVec_;
   int t, team, cols;
   __device__ __forceinline__ int at(int i, int j) const { return kVec ? 8 * (t + i * team) + j : (8 * i + j) * team + t; }
   __device__ __forceinline__ bool has(int i, int j) const { return kVec ? 8 * (t + i * team) < cols : at(i, j) < cols; }
-  // (pointer to a row) -> group i; columns past the row read as 0
-  template <class T> __device__ __forceinline__ void load(const T* row, int i, float (&v)[8]) const {
+  // (pointer to a row) -> group i as it is stored; columns past the row read as 0
+  template <class T> __device__ __forceinline__ Eight<T> fetch(const T* row, int i) const {
+    Eight<T> e = zeros<T>();
     if (kVec) {
-      if (has(i, 0)) {
-        load8(row + at(i, 0), v);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = has(i, j) ? to_f32(row[at(i, j)]) : 0.0f;
-    }
-  }
-  template <class T> __device__ __forceinline__ void store(T* row, int i, const float (&v)[8]) const {
-    if (kVec) {
-      if (has(i, 0)) store8(row + at(i, 0), v);
+      if (has(i, 0)) e = read16(row + at(i, 0));
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (has(i, j)) row[at(i, j)] = from_f32<T>(v[j]);
+        if (has(i, j)) put_value(e, j, row + at(i, j));
     }
+    return e;
+  }
+  template <class T> __device__ __forceinline__ F8 load(const T* row, int i) const { return expand(fetch(row, i)); }
+  template <class T> __device__ __forceinline__ void store(T* row, int i, const F8& v) const {
+    const Eight<T> e = narrow<T>(v);
+    if (kVec) {
+      if (has(i, 0)) write16(row + at(i, 0), e);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (has(i, j)) row[at(i, j)] = value_of(e, j);
+    }
+  }
+  // 1, or 0 where the thread has none of group i: with kVec it has all eight columns or none, and a factor keeps what lies past the
+  // row at 0; without, mask() does so column by column
+  __device__ __forceinline__ float in(int i) const { return !kVec || has(i, 0) ? 1.0f : 0.0f; }
+  __device__ __forceinline__ F8 mask(int i, const F8& a) const {
+    if (kVec) return a;
+    float v[8];
+    unpack8(a, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = has(i, j) ? v[j] : 0.0f;
+    return pack8(v);
   }
   __device__ __forceinline__ int count(int groups) const {        // how many of the row's columns the thread holds
     int n = 0;
@@ -68,53 +205,130 @@ template <bool kVec> struct Columns {
   }
 };
 
+// The same where each warp has a run of 256 kGroups columns, group i eight of them a lane from column first + 256 i on: a thread's
+// groups lie at distances that the compiler knows.
+struct WarpColumns {
+  static constexpr bool kVec = true;
+  int first, cols;
+  __device__ __forceinline__ int at(int i, int j) const { return first + 256 * i + j; }
+  __device__ __forceinline__ bool has(int i, int) const { return first + 256 * i < cols; }
+  __device__ __forceinline__ int count(int groups) const {
+    int n = 0;
+    for (int i = 0; i < groups; ++i) n += has(i, 0) ? 8 : 0;
+    return n;
+  }
+};
+
 __device__ __forceinline__ float warp_total(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+// Sums of four values over a warp in six shuffles instead of twenty: lanes hand over what the others will need.  The sum of the
+// q-th value ends in lanes 8 q .. 8 q + 7.
+__device__ __forceinline__ float warp_total4(float a, float b, float c, float d, int lane) {
+  const bool hi = lane & 16, odd = lane & 8;
+  float x = (hi ? c : a) + __shfl_xor_sync(0xffffffffu, hi ? a : c, 16), y = (hi ? d : b) + __shfl_xor_sync(0xffffffffu, hi ? b : d, 16);
+  x = (odd ? y : x) + __shfl_xor_sync(0xffffffffu, odd ? x : y, 8);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
 
-// A team of warps that works on one row.  `box` is its shared memory, 2 x 32 float2, used in turn, so that one barrier an
+// A team of warps that works on one row.  `box` is its shared memory, 2 x 32 float4, used in turn, so that one barrier an
 // exchange is enough: a warp that writes a half again has left the barrier behind the other half's exchange, in front of which
 // everybody had read this one.
-constexpr int kTeamBox = 64 * sizeof(float2) + 32 * sizeof(float);
+constexpr int kTeamBox = 64 * sizeof(float4) + 32 * sizeof(float);
 struct Team {
   int warps, warp, lane, barrier;      // barrier: a named one of the team's own
-  float2* box;
+  float4* box;
   float* counts;                       // shared: columns that each warp holds
   int turn;
-  float inv_cols, warp_cols;           // 1 / columns of the row; columns that this warp holds
+  float inv_cols, warp_cols, inv_warp_cols;
   // `all`: shared memory of kTeamBox bytes; readers of `counts` come behind the first exchange's barrier
-  template <bool kVec>
-  __device__ __forceinline__ void begin(char* all, int warps_, int warp_, int barrier_, const Columns<kVec>& cols, int groups) {
+  template <class C>
+  __device__ __forceinline__ void begin(char* all, int warps_, int warp_, int barrier_, const C& cols, int groups) {
     warps = warps_;
     warp = warp_;
     lane = threadIdx.x & 31;
     barrier = barrier_;
-    box = reinterpret_cast<float2*>(all);
-    counts = reinterpret_cast<float*>(all + 64 * sizeof(float2));
+    box = reinterpret_cast<float4*>(all);
+    counts = reinterpret_cast<float*>(all + 64 * sizeof(float4));
     turn = 0;
     inv_cols = 1.0f / (float)cols.cols;
     warp_cols = (float)__reduce_add_sync(0xffffffffu, cols.count(groups));
+    inv_warp_cols = warp_cols > 0.0f ? 1.0f / warp_cols : 0.0f;
     if (warps > 1 && lane == 0) counts[warp] = warp_cols;
   }
-  __device__ __forceinline__ void gather(float2 mine) {
-    turn ^= 32;
-    if (lane == 0) box[turn + warp] = mine;
-    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(32 * warps) : "memory");
-  }
-  // sums of both over the team, the same bits in every thread
-  __device__ __forceinline__ float2 sum(float2 v) {
-    v.x = warp_total(v.x);
-    v.y = warp_total(v.y);
-    if (warps == 1) return v;
-    gather(v);
-    v = box[turn];
-    for (int w = 1; w < warps; ++w) {
-      v.x += box[turn + w].x;
-      v.y += box[turn + w].y;
+  __device__ __forceinline__ void meet() { asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(32 * warps) : "memory"); }
+  // Sums over the team of what warp_total4 left: the same bits in every thread.
+  __device__ __forceinline__ float4 exchange(float part) {
+    float4 v;
+    if (warps == 1) {
+      v.x = __shfl_sync(0xffffffffu, part, 0);
+      v.y = __shfl_sync(0xffffffffu, part, 8);
+      v.z = __shfl_sync(0xffffffffu, part, 16);
+      v.w = __shfl_sync(0xffffffffu, part, 24);
+      return v;
     }
+    turn ^= 32;
+    if ((lane & 7) == 0) reinterpret_cast<float*>(&box[turn + warp])[lane >> 3] = part;
+    meet();
+    if (warps <= 4) {
+      v = box[turn];
+      for (int w = 1; w < warps; ++w) {
+        const float4 o = box[turn + w];
+        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+      }
+      return v;
+    }
+    const float4 o = lane < warps ? box[turn + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    part = warp_total4(o.x, o.y, o.z, o.w, lane);
+    v.x = __shfl_sync(0xffffffffu, part, 0);
+    v.y = __shfl_sync(0xffffffffu, part, 8);
+    v.z = __shfl_sync(0xffffffffu, part, 16);
+    v.w = __shfl_sync(0xffffffffu, part, 24);
     return v;
+  }
+  template <int kWarps> __device__ __forceinline__ float4 merged() const {
+    float4 o[kWarps];
+    float n[kWarps], mean = 0.0f, m2 = 0.0f, a = 0.0f, s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      o[w] = box[turn + w];
+      n[w] = counts[w];
+      mean = fmaf(n[w], o[w].w, mean);
+    }
+    mean *= inv_cols;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float off = o[w].w - mean;
+      m2 += fmaf(n[w] * off, off, o[w].x);
+      a += o[w].y;
+      s += fmaf(o[w].y, off, o[w].z);
+    }
+    return make_float4(mean, m2, a, s);
+  }
+  // Each warp's mean of a row with sums around it -- squared deviations m2, and a and the product sum s = sum a (x - mean_w) of another
+  // row a -- become the row's: M2 = sum_w m2_w + n_w (mean_w - mean)^2, S = sum_w s_w + a_w (mean_w - mean).  `part` as warp_total4(m2, a, s, .)
+  // leaves it.  Returns (mean, M2, A, S).
+  __device__ __forceinline__ float4 merge(float mean_w, float part) {
+    if (warps == 1) {
+      const float m2 = __shfl_sync(0xffffffffu, part, 0), a = __shfl_sync(0xffffffffu, part, 8), s = __shfl_sync(0xffffffffu, part, 16);
+      return make_float4(mean_w, m2, a, s);
+    }
+    turn ^= 32;
+    if ((lane & 7) == 0) reinterpret_cast<float*>(&box[turn + warp])[lane >> 3] = lane == 24 ? mean_w : part;
+    meet();
+    if (warps == 2) return merged<2>();
+    if (warps == 3) return merged<3>();
+    if (warps == 4) return merged<4>();
+    const float4 o = lane < warps ? box[turn + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float n = lane < warps ? counts[lane] : 0.0f;
+    const float mean = warp_total(n * o.w) * inv_cols;
+    const float off = o.w - mean;
+    part = warp_total4(fmaf(n * off, off, o.x), o.y, fmaf(o.y, off, o.z), 0.0f, lane);
+    return make_float4(mean, __shfl_sync(0xffffffffu, part, 0), __shfl_sync(0xffffffffu, part, 8), __shfl_sync(0xffffffffu, part, 16));
   }
 };
 
@@ -122,53 +336,31 @@ struct Team {
 __device__ __forceinline__ uint32_t team_max_bits(Team& team, uint32_t bits) {
   bits = __reduce_max_sync(0xffffffffu, bits);
   if (team.warps == 1) return bits;
-  team.gather(make_float2(__uint_as_float(bits), 0.0f));
-  for (int w = 0; w < team.warps; ++w) bits = max(bits, __float_as_uint(team.box[team.turn + w].x));
-  return bits;
+  team.turn ^= 32;
+  if (team.lane == 0) team.box[team.turn + team.warp].x = __uint_as_float(bits);
+  team.meet();
+  return __reduce_max_sync(0xffffffffu, team.lane < team.warps ? __float_as_uint(team.box[team.turn + team.lane].x) : 0u);
 }
 
-// (mean, 1 / sqrt(var + eps)) of a row.  Layer: warps take their own mean and squared deviations from it (two passes over
-// registers) and merge by  M2 = sum_w M2_w + n_w (mean_w - mean)^2.  Rms: mean 0.
+// (mean, 1 / sqrt(var + eps)) of a row, two passes over registers.  Rms: mean 0.
 template <int kGroups, bool kVec>
-__device__ __forceinline__ float2 row_stats(Team& team, const Columns<kVec>& cols, const float (&x)[kGroups][8], bool rms, float eps) {
-  float a = 0.0f;
-  if (rms) {
+__device__ __forceinline__ float2 row_stats(Team& team, const Columns<kVec>& cols, const F8 (&x)[kGroups], bool rms, float eps) {
+  float mean_w = 0.0f, m2 = 0.0f;
+  if (!rms) {
+    float a = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) a = fmaf(x[i][j], x[i][j], a);       // columns past the row hold 0
-    a = team.sum(make_float2(a, 0.0f)).x;
-    return make_float2(0.0f, rsqrtf(a * team.inv_cols + eps));
+    for (int i = 0; i < kGroups; ++i) a += sum8(x[i]);                  // columns past the row hold 0
+    mean_w = warp_total(a) * team.inv_warp_cols;
   }
 #pragma unroll
-  for (int i = 0; i < kGroups; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) a += x[i][j];
-  a = warp_total(a);
-  const float mean_w = a / fmaxf(team.warp_cols, 1.0f);
-  float m2 = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kGroups; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float d = cols.has(i, j) ? x[i][j] - mean_w : 0.0f;
-      m2 = fmaf(d, d, m2);
-    }
+  for (int i = 0; i < kGroups; ++i) {
+    const F8 d = cols.mask(i, add8(x[i], -mean_w * cols.in(i)));
+    m2 += dot8(d, d);
+  }
   m2 = warp_total(m2);
-  float mean = mean_w;
-  if (team.warps > 1) {
-    team.gather(make_float2(a, m2));
-    mean = 0.0f;
-    for (int w = 0; w < team.warps; ++w) mean += team.box[team.turn + w].x;
-    mean *= team.inv_cols;
-    m2 = 0.0f;
-    for (int w = 0; w < team.warps; ++w) {
-      const float2 of = team.box[team.turn + w];
-      const float n = team.counts[w], d = of.x / fmaxf(n, 1.0f) - mean;
-      m2 += fmaf(n * d, d, of.y);
-    }
-  }
-  return make_float2(mean, rsqrtf(m2 * team.inv_cols + eps));
+  if (team.warps == 1) return make_float2(mean_w, rsqrtf(m2 * team.inv_cols + eps));
+  const float4 st = team.merge(mean_w, m2);       // (the other sums' places hold m2 too, and are not looked at)
+  return make_float2(rms ? 0.0f : st.x, rsqrtf(st.y * team.inv_cols + eps));
 }
 
 // A row in 8-bit integers: q = rint(x min(127 / a, FLT_MAX)) with a = max |x|, scale a / 127.  A row with an infinity or a NaN has scale
@@ -186,23 +378,26 @@ __device__ __forceinline__ uint32_t pack_s8(float a, float b, float c, float d) 
   return (uint32_t)(__float2int_rn(a) & 255) | (uint32_t)(__float2int_rn(b) & 255) << 8 | (uint32_t)(__float2int_rn(c) & 255) << 16 |
          (uint32_t)(__float2int_rn(d)) << 24;
 }
-template <int kGroups, bool kVec>
-__device__ __forceinline__ void quantise_row(Team& team, const Columns<kVec>& cols, const float (&x)[kGroups][8], signed char* q, float* scale) {
+template <int kGroups, class C>
+__device__ __forceinline__ void quantise_row(Team& team, const C& cols, const F8 (&x)[kGroups], signed char* q, float* scale) {
   uint32_t most = 0;
+  float v[8];
 #pragma unroll
-  for (int i = 0; i < kGroups; ++i)
+  for (int i = 0; i < kGroups; ++i) {
+    unpack8(x[i], v);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (cols.has(i, j)) most = max(most, abs_bits(x[i][j]));
+      if (cols.has(i, j)) most = max(most, abs_bits(v[j]));
+  }
   most = team_max_bits(team, most);
   const RowScale rs = row_scale(most);
   const bool fine = most < 0x7f800000u;      // 0 * inf is no number
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
-    float v[8];
+    unpack8(x[i], v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = fine ? x[i][j] * rs.inv : 0.0f;
-    if (kVec) {
+    for (int j = 0; j < 8; ++j) v[j] = fine ? v[j] * rs.inv : 0.0f;
+    if (C::kVec) {
       if (cols.has(i, 0)) *reinterpret_cast<uint2*>(q + cols.at(i, 0)) = make_uint2(pack_s8(v[0], v[1], v[2], v[3]), pack_s8(v[4], v[5], v[6], v[7]));
     } else {
 #pragma unroll

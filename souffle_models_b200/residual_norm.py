@@ -173,3 +173,8 @@ def residual_norm_backward(grad_sum: Optional[torch.Tensor], grad_out: Optional[
         ptr(d["branch_bias"]), ptr(d["out_weight"]), ptr(d["out_bias"]), ws.data_ptr(), ws.numel()), stream))
     d["residual"], d["branch"] = dr, dy
     return d
+
+
+def status() -> None:
+    """Synchronises the current stream and raises SouffleError if a device-side wait of one of these calls has expired."""
+    _lib.check(_lib.load().souffle_residual_norm_status(_lib.stream_ptr()))
