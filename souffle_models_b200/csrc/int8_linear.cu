@@ -36,6 +36,7 @@ __global__ void __launch_bounds__(256) souffle_quantise_rows(const T* __restrict
   const Columns<kVec> cols = {(int)(threadIdx.x % (32 * warps_per_row)), 32 * warps_per_row, cols_n};
   Team team;
   team.begin(box, warps_per_row, warp % warps_per_row, 1, cols, 0);
+  if (warps_per_row > 1) team.meet();
   if (kGroups * 256 * warps_per_row >= cols_n) {
     F8 v[kGroups];
 #pragma unroll

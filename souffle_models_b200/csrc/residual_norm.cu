@@ -3,8 +3,9 @@
 // Memory-bound: forward reads r and y and writes s and o (4 C values a row), backward reads r, y, ds, do and writes dr, dy (6 C
 // values a row); nothing else of a row leaves the registers, and s is computed again in the backward pass, unrounded, instead of
 // being read.  A row belongs to a team of warps and lies in its registers between the passes over it.
-#include <float.h>
 #include <string.h>
+
+#include <type_traits>
 
 #include "host_common.h"
 #include "row_io.cuh"
@@ -64,6 +65,7 @@ __global__ void __launch_bounds__(256) souffle_residual_norm_any(const NormArgs 
   const Columns<kVec> cols = {(int)(threadIdx.x % (32 * warps_per_row)), 32 * warps_per_row, a.cols};
   Team team;
   team.begin(box, warps_per_row, warp % warps_per_row, 1, cols, kGroups);
+  if (warps_per_row > 1) team.meet();
 
   F8 u[kGroups], h[kGroups];
   const T* y = static_cast<const T*>(a.y) + row * a.y_stride;
@@ -174,9 +176,11 @@ template <int kOperands> struct RowRing {
     fence_proxy_async_smem();
     for (int i = 0; i < slots && left > 0; ++i) ask(i);
   }
-  __device__ __forceinline__ const char* wait(const WaitCtl& c) {
-    mbar_wait_hot(bars + 8 * slot, parity, c, 1);
-    return at0 + slot * operands * row_bytes;
+  // the row `ahead` (0 or 1) behind the next one to be released
+  __device__ __forceinline__ const char* wait(const WaitCtl& c, int ahead = 0) {
+    const int s = slot + ahead < slots ? slot + ahead : slot + ahead - slots;
+    mbar_wait_hot(bars + 8 * s, slot + ahead < slots ? parity : parity ^ 1, c, 1);
+    return at0 + s * operands * row_bytes;
   }
   __device__ __forceinline__ void release(bool lane) {      // behind a barrier of those that have read the slot
     if (lane && left > 0) ask(slot);
@@ -255,11 +259,12 @@ __global__ void __launch_bounds__(768, 1) souffle_residual_norm_rows(const NormA
     for (int i = 0; i < kGroups; ++i) m2 += dot8(x[i], x[i]);
     m2 = warp_total(m2);
     if (team.warps > 1) {
-      const float4 st = team.merge(mean_w, m2);
-      m2 = st.y;
+      float4 st[1];
+      team.merge<1>({mean_w}, {m2}, st);
+      m2 = st[0].y;
       if (!rms) {
 #pragma unroll
-        for (int i = 0; i < kGroups; ++i) x[i] = add8(x[i], has(i) ? mean_w - st.x : 0.0f);
+        for (int i = 0; i < kGroups; ++i) x[i] = add8(x[i], has(i) ? mean_w - st[0].x : 0.0f);
       }
     }
     const float rstd = rsqrtf(m2 * team.inv_cols + eps);
@@ -333,10 +338,15 @@ struct NormGradArgs {
   const void *ds, *dout;
   void *dr, *dy, *dgate, *dvec[4];     // dvec: SUM_W1 .. SUM_B2
   float *part, *slots;                 // [ctas][SUMS][cols], [teams][2][cols]
-  int teams;                           // of the whole grid
+  int teams, rows_each, rows_over;     // of the whole grid; rows / teams and rows % teams
 };
 
-__device__ __forceinline__ int first_row(long long team, int rows, int teams) { return (int)(team * rows / teams); }
+// Rows are dealt out evenly, the first rows % teams teams having one more.
+__device__ __forceinline__ int first_row(int team, const NormGradArgs& g) { return team * g.rows_each + min(team, g.rows_over); }
+__device__ __forceinline__ int team_of_row(int row, const NormGradArgs& g) {
+  const int more = g.rows_over * (g.rows_each + 1);
+  return row < more ? row / (g.rows_each + 1) : g.rows_over + (row - more) / g.rows_each;
+}
 
 constexpr int kGradWarps = 12;
 // kSharedSums: the sums lie in shared memory, [SUMS][8][threads], where 1024 threads leave no registers for them.
@@ -349,6 +359,7 @@ __global__ void __launch_bounds__(kSharedSums ? 1024 : 32 * kGradWarps, 1) souff
   const Columns<kVec> cols = {(int)(threadIdx.x % (32 * warps_per_row)), 32 * warps_per_row, a.cols};
   Team team;
   team.begin(smem + mine * kTeamBox, warps_per_row, warp % warps_per_row, 1 + mine, cols, 1);
+  __syncthreads();
   float* sums = reinterpret_cast<float*>(smem + teams * kTeamBox);
   const float in = cols.in(0);
 
@@ -393,7 +404,7 @@ __global__ void __launch_bounds__(kSharedSums ? 1024 : 32 * kGradWarps, 1) souff
     return pack8(v);
   };
 
-  const int begin = first_row(id, a.rows, g.teams), end = first_row(id + 1LL, a.rows, g.teams);
+  const int begin = first_row(id, g), end = first_row(id + 1, g);
   const int per_gate = a.gate ? a.rows / a.gate_rows : 0x7fffffff;
   int gate_at = a.gate ? begin / per_gate : 0, gate_first = gate_at * per_gate;       // the row's gate, and that one's first row
   const bool n1 = a.branch_norm != SOUFFLE_NORM_NONE, n2 = a.out_norm != SOUFFLE_NORM_NONE;
@@ -420,7 +431,9 @@ __global__ void __launch_bounds__(kSharedSums ? 1024 : 32 * kGradWarps, 1) souff
     if (n1) {                          // y becomes yhat, u = N1(y)
       const float mean_w = rms1 ? 0.0f : warp_total(sum8(y)) * team.inv_warp_cols;
       y = cols.mask(0, add8(y, -mean_w * in));
-      const float4 st = team.merge(mean_w, warp_total(dot8(y, y)));
+      float4 sts[1];
+      team.merge<1>({mean_w}, {warp_total(dot8(y, y))}, sts);
+      const float4 st = sts[0];
       rstd1 = rsqrtf(st.y * team.inv_cols + a.eps1);
       if (team.warps > 1 && !rms1) y = cols.mask(0, add8(y, (mean_w - st.x) * in));
       y = mul8(y, rstd1);
@@ -435,7 +448,9 @@ __global__ void __launch_bounds__(kSharedSums ? 1024 : 32 * kGradWarps, 1) souff
       h = cols.mask(0, add8(h, -mean_w * in));
       F8 e = expand(o_raw);
       if (a.w2) e = mul8(e, load_param(cols, a, a.w2, 0, 0));
-      const float4 st = team.merge(mean_w, warp_total4(dot8(h, h), sum8(e), dot8(e, h), 0.0f, team.lane));
+      float4 sts[1];
+      team.merge<1>({mean_w}, {warp_total4(dot8(h, h), sum8(e), dot8(e, h), 0.0f, team.lane)}, sts);
+      const float4 st = sts[0];
       const float rstd = rsqrtf(st.y * team.inv_cols + a.eps2);
       if (team.warps > 1 && !rms2) h = cols.mask(0, add8(h, (mean_w - st.x) * in));
       h = mul8(h, rstd);
@@ -454,7 +469,9 @@ __global__ void __launch_bounds__(kSharedSums ? 1024 : 32 * kGradWarps, 1) souff
       if (g.dvec[SUM_W1]) add(SUM_W1, d, y);
       if (g.dvec[SUM_B1]) add1(SUM_B1, d);
       if (a.w1) d = mul8(d, load_param(cols, a, a.w1, 0, 0));
-      const float4 m = team.exchange(warp_total4(sum8(d), dot8(d, y), 0.0f, 0.0f, team.lane));
+      float4 ms[1];
+      team.exchange<1>({warp_total4(sum8(d), dot8(d, y), 0.0f, 0.0f, team.lane)}, ms);
+      const float4 m = ms[0];
       d = fma8(y, -m.y * team.inv_cols, d);
       if (!rms1) d = add8(d, -m.x * team.inv_cols);
       d = mul8(d, rstd1);
@@ -472,6 +489,7 @@ __global__ void __launch_bounds__(kSharedSums ? 1024 : 32 * kGradWarps, 1) souff
     }
   }
 
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // The teams of the CTA, one sum at a time: each team lays its columns down, every thread adds up some.
   const bool have[SUMS] = {g.dvec[SUM_W1] != nullptr, g.dvec[SUM_B1] != nullptr, g.dvec[SUM_W2] != nullptr, g.dvec[SUM_B2] != nullptr,
                            g.dgate && a.gate_rows == 1};
@@ -495,10 +513,15 @@ __global__ void __launch_bounds__(kSharedSums ? 1024 : 32 * kGradWarps, 1) souff
   }
 }
 
-// The same with rows through the ring, eight columns a lane; widths up to 256 kGradWarps.
-constexpr int kGradRowWarps = 16;
-template <class T, bool kFull, bool kN1, bool kN2>
-__global__ void __launch_bounds__(32 * kGradRowWarps, 1) souffle_residual_norm_grad_rows(const NormGradArgs g, const RowPlan p) {
+// The same with rows through the ring, eight columns a lane.  kTwo: two rows at a time, whose chains of shuffles and exchanges
+// overlap and which share what is read and decided for both; with two norms that takes 168 registers, so that a row has at most twelve
+// warps.  It is for a norm on the branch, where a row is three or four dependent exchanges (8192 x 768 fp16, both norms, 42.9 -> 34.2 us; 2048
+// bf16 107 -> 96); without one, one row at a time and sixteen warps are as fast or faster (16384 x 256 fp16 20.6 -> 19.5, 8192 x 2048
+// fp32 85 -> 74.6).  Two rows hold two slots, so that fewer than kTwoSlots leave none for the rows behind them.
+constexpr int kTwoSlots = 4;
+constexpr int grad_row_warps(bool both_norms, bool two) { return both_norms && two ? 12 : 16; }
+template <class T, bool kFull, bool kN1, bool kN2, bool kTwo>
+__global__ void __launch_bounds__(32 * grad_row_warps(kN1 && kN2, kTwo), 1) souffle_residual_norm_grad_rows(const NormGradArgs g, const RowPlan p) {
   extern __shared__ __align__(128) char smem[];
   const NormArgs& a = g.f;
   RowCtl& ctl = *reinterpret_cast<RowCtl*>(smem);
@@ -510,7 +533,7 @@ __global__ void __launch_bounds__(32 * kGradRowWarps, 1) souffle_residual_norm_g
   float* gate_s = reinterpret_cast<float*>(own + team_gate_at()) + plane_at(c);
   const bool has = kFull || c < n;
   float* vec = reinterpret_cast<float*>(smem + p.vectors);
-  const int begin = first_row(id, a.rows, g.teams), end = first_row(id + 1LL, a.rows, g.teams);
+  const int begin = first_row(id, g), end = first_row(id + 1, g);
   const bool have_r = a.r != nullptr, have_ds = g.ds != nullptr, have_gate = a.gate != nullptr;
   RowRing<4> ring;                             // y, r, do, ds
   ring.step[0] = a.y_stride * (long long)sizeof(T);
@@ -521,7 +544,7 @@ __global__ void __launch_bounds__(32 * kGradRowWarps, 1) souffle_residual_norm_g
   ring.from[1] = kN2 && have_r ? static_cast<const char*>(a.r) + begin * ring.step[1] : nullptr;
   ring.from[2] = kN2 ? static_cast<const char*>(g.dout) + begin * ring.step[2] : nullptr;
   ring.from[3] = have_ds ? static_cast<const char*>(g.ds) + begin * ring.step[3] : nullptr;
-  ring.at0 = own + team_ring_at(n, have_gate);
+  ring.at0 = own + team_ring_at(n, true);
   ring.bars = smem_u32(own + kTeamBox);
   ring.parity = 0;
   ring.slots = p.slots, ring.row_bytes = p.row_bytes, ring.operands = p.operands, ring.slot = 0;
@@ -541,92 +564,146 @@ __global__ void __launch_bounds__(32 * kGradRowWarps, 1) souffle_residual_norm_g
   for (int k = 0; k < SUMS; ++k) acc[k] = all8(0.0f);
   const int per_gate = have_gate ? a.rows / a.gate_rows : 0x7fffffff;
   int gate_at = have_gate ? begin / per_gate : 0, gate_first = gate_at * per_gate;       // the row's gate, and that one's first row
-  bool gate_new = have_gate;
-  const bool rms1 = a.branch_norm == SOUFFLE_NORM_RMS, rms2 = a.out_norm == SOUFFLE_NORM_RMS;
+  const float layer1 = a.branch_norm == SOUFFLE_NORM_RMS ? 0.0f : 1.0f, layer2 = a.out_norm == SOUFFLE_NORM_RMS ? 0.0f : 1.0f;
   T *dr = static_cast<T*>(g.dr) + begin * g.dr_stride + c, *dy = static_cast<T*>(g.dy) + begin * g.dy_stride + c;
-  for (int row = begin; row < end; ++row) {
-    if (gate_new && has) write_plane(gate_s, mul8(read_param(a, a.gate, (long long)gate_at * n + c), a.beta));       // it is read by who wrote it
-    gate_new = false;
-    const char* slot = ring.wait(ctl.wait) + c * (int)sizeof(T);
-    F8 y = has ? expand(read16(reinterpret_cast<const T*>(slot))) : all8(0.0f), u = y;
-    float rstd1 = 1.0f;
-    if (kN1) {                         // y becomes yhat, u = N1(y)
-      const float mean_w = rms1 ? 0.0f : warp_total(sum8(y)) * team.inv_warp_cols;
-      if (!rms1) y = add8(y, has ? -mean_w : 0.0f);
-      float m2 = warp_total(dot8(y, y));
-      if (team.warps > 1) {
-        const float4 st = team.merge(mean_w, m2);
-        m2 = st.y;
-        if (!rms1) y = add8(y, has ? mean_w - st.x : 0.0f);
+  const int at_r = have_r ? ring.row_bytes : 0, at_do = ring.row_bytes + at_r, at_ds = kN2 ? at_do + ring.row_bytes : ring.row_bytes;
+  const float alpha_r = have_r ? a.alpha : 0.0f;       // without residual, 0 times the branch (an infinity there leaves no number either way)
+  auto lay_gate = [&] {                // by who reads it
+    if (has && have_gate) write_plane(gate_s, mul8(read_param(a, a.gate, (long long)gate_at * n + c), a.beta));
+  };
+  lay_gate();
+
+  // kRows rows that share a gate
+  auto rows_of = [&](auto rows_c) {
+    constexpr int kRows = decltype(rows_c)::value;
+    const char* slot[kRows];           // y; r, do and ds, as many of them as there are
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) slot[i] = ring.wait(ctl.wait, i) + c * (int)sizeof(T);
+    auto operand = [&](int i, int at) { return has ? expand(read16(reinterpret_cast<const T*>(slot[i] + at))) : all8(0.0f); };
+    auto plane8 = [&](const float* at) { return has ? read_plane(at) : all8(0.0f); };
+    // what is in shared memory is read again where it is needed again: the five sums leave no registers to keep it
+    F8 y[kRows], d[kRows];
+    float rstd1[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) y[i] = operand(i, 0);
+    if (kN1) {                         // y becomes yhat
+      float mean_w[kRows], part[kRows];
+      float4 st[kRows];
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) mean_w[i] = warp_total(sum8(y[i])) * team.inv_warp_cols * layer1;
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        y[i] = add8(y[i], has ? -mean_w[i] : 0.0f);
+        part[i] = warp_total(dot8(y[i], y[i]));
       }
-      rstd1 = rsqrtf(m2 * team.inv_cols + a.eps1);
-      y = mul8(y, rstd1);
-      if (has) u = fma8(y, read_plane(w1), read_plane(b1));
+      team.merge(mean_w, part, st);
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        rstd1[i] = rsqrtf(st[i].y * team.inv_cols + a.eps1);
+        const float r = has ? rstd1[i] : 0.0f;
+        y[i] = fma8(y[i], r, all8((mean_w[i] - st[i].x) * r));
+      }
     }
-    F8 d = all8(0.0f);
-    if (kN2) {                         // h becomes hhat, d the gradient of s
-      F8 h = have_gate ? (has ? mul8(u, read_plane(gate_s)) : u) : mul8(u, a.beta), e = d, o = d;
-      const char* at = slot + ring.row_bytes;
-      if (has) {
-        if (have_r) {
-          h = fma8(expand(read16(reinterpret_cast<const T*>(at))), a.alpha, h);
-          at += ring.row_bytes;
+    if (kN2) {
+      F8 h[kRows], e[kRows];           // h becomes hhat
+      float mean_w[kRows], part[kRows];
+      float4 st[kRows];
+      {
+        const F8 w = kN1 ? plane8(w1) : all8(1.0f), b = kN1 ? plane8(b1) : all8(0.0f), gt = have_gate ? plane8(gate_s) : all8(a.beta), v = plane8(w2);
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          h[i] = fma8(operand(i, at_r), alpha_r, mul8(kN1 ? fma8(y[i], w, b) : y[i], gt));
+          e[i] = mul8(operand(i, at_do), v);
         }
-        o = expand(read16(reinterpret_cast<const T*>(at)));
-        if (have_ds) d = expand(read16(reinterpret_cast<const T*>(at + ring.row_bytes)));
-        e = mul8(o, read_plane(w2));
       }
-      const float mean_w = rms2 ? 0.0f : warp_total(sum8(h)) * team.inv_warp_cols;
-      if (!rms2) h = add8(h, has ? -mean_w : 0.0f);
-      const float4 st = team.merge(mean_w, warp_total4(dot8(h, h), sum8(e), dot8(e, h), 0.0f, team.lane));
-      const float rstd = rsqrtf(st.y * team.inv_cols + a.eps2);
-      if (!rms2 && team.warps > 1) h = add8(h, has ? mean_w - st.x : 0.0f);
-      h = mul8(h, rstd);
-      acc[SUM_W2] = fma8(o, h, acc[SUM_W2]);
-      acc[SUM_B2] = add8(acc[SUM_B2], o);
-      // d += rstd (e - mean e - hhat mean (e hhat))
-      e = fma8(h, -rstd * st.w * team.inv_cols, e);
-      if (!rms2) e = add8(e, has ? -st.z * team.inv_cols : 0.0f);
-      d = fma8(e, rstd, d);
-    } else if (have_ds && has) {
-      d = expand(read16(reinterpret_cast<const T*>(slot + ring.row_bytes)));
-    }
-    if (g.dr && has) write16(dr, narrow<T>(mul8(d, a.alpha)));
-    if (g.dgate) acc[SUM_GATE] = fma8(d, u, acc[SUM_GATE]);         // beta comes in at the end
-    if (have_gate) {
-      if (has) d = mul8(d, read_plane(gate_s));
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) mean_w[i] = warp_total(sum8(h[i])) * team.inv_warp_cols * layer2;
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        h[i] = add8(h[i], has ? -mean_w[i] : 0.0f);
+        part[i] = warp_total4(dot8(h[i], h[i]), sum8(e[i]), dot8(e[i], h[i]), 0.0f, team.lane);
+      }
+      team.merge(mean_w, part, st);
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const float rstd = rsqrtf(st[i].y * team.inv_cols + a.eps2), r = has ? rstd : 0.0f;
+        h[i] = fma8(h[i], r, all8((mean_w[i] - st[i].x) * r));
+        // d = ds + rstd (e - mean e - hhat mean (e hhat))
+        e[i] = fma8(h[i], -rstd * st[i].w * team.inv_cols, add8(e[i], has ? -st[i].z * team.inv_cols * layer2 : 0.0f));
+        const F8 o = operand(i, at_do);
+        acc[SUM_W2] = fma8(o, h[i], acc[SUM_W2]);
+        acc[SUM_B2] = add8(acc[SUM_B2], o);
+        d[i] = mul8(e[i], rstd);
+      }
+      if (have_ds) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) d[i] = add8(d[i], operand(i, at_ds));
+      }
     } else {
-      d = mul8(d, a.beta);
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) d[i] = operand(i, at_ds);
+    }
+    if (g.dr && has) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) write16(dr + i * g.dr_stride, narrow<T>(mul8(d[i], a.alpha)));
+    }
+    {
+      const F8 w = kN1 ? plane8(w1) : all8(1.0f), b = kN1 ? plane8(b1) : all8(0.0f), gt = have_gate ? plane8(gate_s) : all8(a.beta);
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        if (g.dgate) acc[SUM_GATE] = fma8(d[i], kN1 ? fma8(y[i], w, b) : y[i], acc[SUM_GATE]);         // beta comes in at the end
+        d[i] = mul8(d[i], gt);
+        if (kN1) {
+          acc[SUM_W1] = fma8(d[i], y[i], acc[SUM_W1]);
+          acc[SUM_B1] = add8(acc[SUM_B1], d[i]);
+          d[i] = mul8(d[i], w);
+        }
+      }
     }
     if (kN1) {
-      acc[SUM_W1] = fma8(d, y, acc[SUM_W1]);
-      acc[SUM_B1] = add8(acc[SUM_B1], d);
-      if (has) d = mul8(d, read_plane(w1));
-      const float4 m = team.exchange(warp_total4(sum8(d), dot8(d, y), 0.0f, 0.0f, team.lane));
-      d = fma8(y, -m.y * team.inv_cols, d);
-      if (!rms1) d = add8(d, -m.x * team.inv_cols);
-      d = mul8(d, rstd1);
+      float part[kRows];
+      float4 m[kRows];
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) part[i] = warp_total4(sum8(d[i]), dot8(d[i], y[i]), 0.0f, 0.0f, team.lane);
+      team.exchange(part, m);
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const float r = rstd1[i] * team.inv_cols;
+        d[i] = fma8(y[i], -m[i].y * r, add8(mul8(d[i], rstd1[i]), -m[i].x * r * layer1));
+      }
     }
     if (team.warps == 1) __syncwarp();
-    else if (!kN1) team.meet();        // (behind the exchange everybody has read the slot)
-    ring.release(t == 0);
-    if (g.dy && has) write16(dy, narrow<T>(d));
-    dr += g.dr_stride;
-    dy += g.dy_stride;
-    const bool last_of_gate = row + 1 - gate_first == per_gate;
-    if (g.dgate && a.gate_rows > 1 && (last_of_gate || row + 1 == end)) {
+    else if (!kN1) team.meet();        // (behind the exchange everybody has read the slots)
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) ring.release(t == 0);
+    if (g.dy && has) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) write16(dy + i * g.dy_stride, narrow<T>(d[i]));
+    }
+    dr += kRows * g.dr_stride;
+    dy += kRows * g.dy_stride;
+  };
+
+  for (int row = begin; row < end;) {
+    const bool two = kTwo && row + 1 < end && row + 1 - gate_first < per_gate && p.slots >= kTwoSlots;
+    if (two) rows_of(std::integral_constant<int, kTwo ? 2 : 1>());
+    else rows_of(std::integral_constant<int, 1>());
+    row += two ? 2 : 1;
+    const bool gate_done = row - gate_first == per_gate;
+    if (g.dgate && a.gate_rows > 1 && (gate_done || row == end)) {
       const F8 v = mul8(acc[SUM_GATE], a.beta);
       acc[SUM_GATE] = all8(0.0f);
-      if (gate_first >= begin && last_of_gate) store_param(cols, a, g.dgate, gate_at, v);
+      if (gate_first >= begin && gate_done) store_param(cols, a, g.dgate, gate_at, v);
       else cols.store(g.slots + (2LL * id + (gate_first > begin)) * n, 0, v);
     }
-    if (last_of_gate) {
+    if (gate_done) {
       ++gate_at;
       gate_first += per_gate;
-      gate_new = have_gate;
+      if (row < end) lay_gate();
     }
   }
 
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");       // the kernel that adds the CTAs' sums may be brought in
   // the teams of the CTA, one sum at a time, in what was the rings and vectors
   float* sums = reinterpret_cast<float*>(smem + 64);
 #pragma unroll
@@ -655,44 +732,56 @@ __global__ void __launch_bounds__(32 * kGradRowWarps, 1) souffle_residual_norm_g
 // Adds up what the CTAs left.  y < 4: a vector's sum; y = 4: the one gate row's; y >= SUMS: that of a gate whose rows several teams
 // shared (any other gate was written by its one team): gate y - SUMS, or, where there are more gates than teams, the gate whose
 // last rows are team y - SUMS's.
+// kWide: four neighbouring columns a thread.
 constexpr int kFinishLanes = 8;
-template <class P>
+template <class P, bool kWide>
 __global__ void __launch_bounds__(32 * kFinishLanes) souffle_residual_norm_grad_sums(const NormGradArgs g, int ctas) {
-  __shared__ float sm[kFinishLanes][33];
+  constexpr int kW = kWide ? 4 : 1;
+  __shared__ float sm[kFinishLanes][32 * kW + 4];
+  asm volatile("griddepcontrol.wait;" ::: "memory");       // its blocks may be there before the rows' kernel has ended
   const NormArgs& a = g.f;
-  const int cx = threadIdx.x & 31, lane = threadIdx.x >> 5, c = blockIdx.x * 32 + cx, k = blockIdx.y;
+  const int cx = (threadIdx.x & 31) * kW, lane = threadIdx.x >> 5, c = blockIdx.x * 32 * kW + cx, k = blockIdx.y;
   P* to;
-  float v = 0.0f;
+  float v[kW] = {};
+  auto add = [&](const float* from) {
+    if (kWide) {
+      const float4 x = *reinterpret_cast<const float4*>(from + c);
+      v[0] += x.x, v[kW - 3] += x.y, v[kW - 2] += x.z, v[kW - 1] += x.w;
+    } else {
+      v[0] += from[c];
+    }
+  };
   if (k < SUMS) {
     to = static_cast<P*>(k < SUM_GATE ? g.dvec[k] : a.gate_rows == 1 ? g.dgate : nullptr);
     if (!to) return;
     if (c < a.cols)
 #pragma unroll 8
-      for (int i = lane; i < ctas; i += kFinishLanes) v += g.part[((long long)i * SUMS + k) * a.cols + c];
+      for (int i = lane; i < ctas; i += kFinishLanes) add(g.part + ((long long)i * SUMS + k) * a.cols);
   } else {
     const int per_gate = a.rows / a.gate_rows;
     int gate = k - SUMS;
     if (a.gate_rows > g.teams) {
-      const int begin = first_row(k - SUMS, a.rows, g.teams), end = first_row(k - SUMS + 1LL, a.rows, g.teams);
+      const int begin = first_row(k - SUMS, g), end = first_row(k - SUMS + 1, g);
       gate = begin / per_gate;
       if (begin == end || gate * per_gate == begin || (gate + 1) * per_gate > end) return;
     }
     const int first = gate * per_gate, last = first + per_gate - 1;
-    const int t0 = (int)(((first + 1LL) * g.teams - 1) / a.rows), t1 = (int)(((last + 1LL) * g.teams - 1) / a.rows);     // their teams
+    const int t0 = team_of_row(first, g), t1 = team_of_row(last, g);
     if (t0 == t1) return;
     to = static_cast<P*>(g.dgate) + (long long)gate * a.cols;
     if (c < a.cols)
 #pragma unroll 2
-      for (int t = t0 + lane; t <= t1; t += kFinishLanes) {
-        const int from = first_row(t, a.rows, g.teams);
-        if (from < first_row(t + 1LL, a.rows, g.teams)) v += g.slots[(2LL * t + (first > from)) * a.cols + c];
-      }
+      for (int t = t0 + lane; t <= t1; t += kFinishLanes) add(g.slots + (2LL * t + (first > first_row(t, g))) * a.cols);
   }
-  sm[lane][cx] = v;
+#pragma unroll
+  for (int j = 0; j < kW; ++j) sm[lane][cx + j] = v[j];
   __syncthreads();
-  if (lane || c >= a.cols) return;
-  for (int i = 1; i < kFinishLanes; ++i) v += sm[i][cx];
-  to[c] = from_f32<P>(v);
+  const int out = threadIdx.x, at = blockIdx.x * 32 * kW + out;
+  if (out >= 32 * kW || at >= a.cols) return;
+  float sum = sm[0][out];
+#pragma unroll
+  for (int i = 1; i < kFinishLanes; ++i) sum += sm[i][out];
+  to[at] = from_f32<P>(sum);
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------
@@ -852,12 +941,25 @@ static int finish_sums(const NormGradArgs& g, int ctas, cudaStream_t st) {
   bool any = g.dgate && (g.f.gate_rows == 1 || shared_gates);
   for (void* p : g.dvec) any = any || p;
   if (!any) return SOUFFLE_OK;
-  const dim3 grid((g.f.cols + 31) / 32, SUMS + shared_gates);
-  if (g.f.param_dtype == SOUFFLE_F32) souffle_residual_norm_grad_sums<float><<<grid, 32 * kFinishLanes, 0, st>>>(g, ctas);
-  else if (g.f.param_dtype == SOUFFLE_F16) souffle_residual_norm_grad_sums<__half><<<grid, 32 * kFinishLanes, 0, st>>>(g, ctas);
-  else souffle_residual_norm_grad_sums<__nv_bfloat16><<<grid, 32 * kFinishLanes, 0, st>>>(g, ctas);
-  SF_CUDA(cudaGetLastError());
-  return SOUFFLE_OK;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  const bool wide = g.f.cols % 4 == 0;         // rows of sums then begin on 16-byte boundaries
+  const int per_block = wide ? 128 : 32;
+  cfg.gridDim = dim3((g.f.cols + per_block - 1) / per_block, SUMS + shared_gates);
+  cfg.blockDim = dim3(32 * kFinishLanes);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  auto go = [&](auto fn) -> int {
+    SF_CUDA(cudaLaunchKernelEx(&cfg, fn, g, ctas));
+    return SOUFFLE_OK;
+  };
+  if (g.f.param_dtype == SOUFFLE_F32) return wide ? go(souffle_residual_norm_grad_sums<float, true>) : go(souffle_residual_norm_grad_sums<float, false>);
+  if (g.f.param_dtype == SOUFFLE_F16) return wide ? go(souffle_residual_norm_grad_sums<__half, true>) : go(souffle_residual_norm_grad_sums<__half, false>);
+  return wide ? go(souffle_residual_norm_grad_sums<__nv_bfloat16, true>) : go(souffle_residual_norm_grad_sums<__nv_bfloat16, false>);
 }
 
 template <class T, bool kVec, bool kSharedSums>
@@ -870,16 +972,25 @@ static int backward_any(const NormGradArgs& g, const GradGrid& gg, cudaStream_t 
   SF_CUDA(cudaGetLastError());
   return SOUFFLE_OK;
 }
-template <class T, bool kFull, bool kN1, bool kN2>
+template <class T, bool kFull, bool kN1, bool kN2, bool kTwo>
 static int backward_rows(const NormGradArgs& g, const RowPlan& p, int grid, int smem, int dev, cudaStream_t st) {
   static bool ready[kMaxDevices];
-  return launch_rows(souffle_residual_norm_grad_rows<T, kFull, kN1, kN2>, g, p, grid, smem, dev, ready, st);
+  return launch_rows(souffle_residual_norm_grad_rows<T, kFull, kN1, kN2, kTwo>, g, p, grid, smem, dev, ready, st);
 }
 template <class T, bool kFull>
 static int backward_rows(const NormGradArgs& g, const RowPlan& p, int grid, int smem, int dev, cudaStream_t st) {
   const bool n1 = g.f.branch_norm != SOUFFLE_NORM_NONE, n2 = g.f.out_norm != SOUFFLE_NORM_NONE;
-  if (n1) return n2 ? backward_rows<T, kFull, true, true>(g, p, grid, smem, dev, st) : backward_rows<T, kFull, true, false>(g, p, grid, smem, dev, st);
-  return n2 ? backward_rows<T, kFull, false, true>(g, p, grid, smem, dev, st) : backward_rows<T, kFull, false, false>(g, p, grid, smem, dev, st);
+  if (n1 && n2)
+    return p.warps <= grad_row_warps(true, true) ? backward_rows<T, kFull, true, true, true>(g, p, grid, smem, dev, st)
+                                                 : backward_rows<T, kFull, true, true, false>(g, p, grid, smem, dev, st);
+  if (n1) return backward_rows<T, kFull, true, false, true>(g, p, grid, smem, dev, st);
+  return n2 ? backward_rows<T, kFull, false, true, false>(g, p, grid, smem, dev, st) : backward_rows<T, kFull, false, false, false>(g, p, grid, smem, dev, st);
+}
+
+static void deal_rows(NormGradArgs& g, int teams) {
+  g.teams = teams;
+  g.rows_each = g.f.rows / teams;
+  g.rows_over = g.f.rows % teams;
 }
 
 // `g` without the workspace's layout, which depends on the grid.
@@ -889,18 +1000,20 @@ static int backward_launch(NormGradArgs& g, bool vec, float* workspace, int sms,
   int groups, grid, smem, ctas, rc;
   const bool n1 = g.f.branch_norm != SOUFFLE_NORM_NONE, n2 = g.f.out_norm != SOUFFLE_NORM_NONE;
   g.part = workspace;
-  if (vec && row_plan(g.f.rows, g.f.cols, sizeof(T), 1 + (n2 && g.f.r) + n2 + (g.ds != nullptr), g.f.gate, 2 * n1 + n2, 1, kGradRowWarps, sms, &p, &groups,
-                      &grid, &smem)) {
+  const auto plan = [&](int warps) {
+    return row_plan(g.f.rows, g.f.cols, sizeof(T), 1 + (n2 && g.f.r) + n2 + (g.ds != nullptr), true, 2 * n1 + n2, 1, warps, sms, &p, &groups, &grid, &smem);
+  };
+  if (vec && (plan(grad_row_warps(n1 && n2, n1)) || plan(grad_row_warps(n1 && n2, false)))) {
     // behind the rows the teams' sums lie in the rings' place
     if (p.teams > 1 && smem < 64 + p.teams * plane_floats(g.f.cols) * 4) smem = 64 + p.teams * plane_floats(g.f.cols) * 4;
     ctas = grid;
-    g.teams = p.total_teams;
+    deal_rows(g, p.total_teams);
     g.slots = g.part + (size_t)ctas * SUMS * g.f.cols;
     rc = g.f.cols == 256 * p.warps ? backward_rows<T, true>(g, p, grid, smem, dev, st) : backward_rows<T, false>(g, p, grid, smem, dev, st);
   } else {
     const GradGrid gg = grad_grid(g.f.rows, g.f.cols, sms);
     ctas = gg.ctas;
-    g.teams = gg.ctas * gg.per_cta;
+    deal_rows(g, gg.ctas * gg.per_cta);
     g.slots = g.part + (size_t)ctas * SUMS * g.f.cols;
     if (gg.warps > kGradWarps) rc = vec ? backward_any<T, true, true>(g, gg, st) : backward_any<T, false, true>(g, gg, st);
     else rc = vec ? backward_any<T, true, false>(g, gg, st) : backward_any<T, false, false>(g, gg, st);

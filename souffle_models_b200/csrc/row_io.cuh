@@ -235,17 +235,18 @@ __device__ __forceinline__ float warp_total4(float a, float b, float c, float d,
   return x;
 }
 
-// A team of warps that works on one row.  `box` is its shared memory, 2 x 32 float4, used in turn, so that one barrier an
-// exchange is enough: a warp that writes a half again has left the barrier behind the other half's exchange, in front of which
-// everybody had read this one.
-constexpr int kTeamBox = 64 * sizeof(float4) + 32 * sizeof(float);
+// A team of warps that works on one row, or on two side by side.  `box` is its shared memory, 2 x 2 x 32 float4 (turn, row, warp), the two
+// turns used alternately, so that one barrier an exchange is enough: a warp that writes a half again has left the barrier behind the
+// other half's exchange, in front of which everybody had read this one.  Up to four warps read four entries without asking how many
+// there are: those of absent warps hold zeros.
+constexpr int kTeamBox = 128 * sizeof(float4) + 32 * sizeof(float);
 struct Team {
   int warps, warp, lane, barrier;      // barrier: a named one of the team's own
   float4* box;
   float* counts;                       // shared: columns that each warp holds
   int turn;
   float inv_cols, warp_cols, inv_warp_cols;
-  // `all`: shared memory of kTeamBox bytes; readers of `counts` come behind the first exchange's barrier
+  // `all`: shared memory of kTeamBox bytes; to be followed by a barrier of the CTA
   template <class C>
   __device__ __forceinline__ void begin(char* all, int warps_, int warp_, int barrier_, const C& cols, int groups) {
     warps = warps_;
@@ -253,82 +254,85 @@ struct Team {
     lane = threadIdx.x & 31;
     barrier = barrier_;
     box = reinterpret_cast<float4*>(all);
-    counts = reinterpret_cast<float*>(all + 64 * sizeof(float4));
+    counts = reinterpret_cast<float*>(all + 128 * sizeof(float4));
     turn = 0;
     inv_cols = 1.0f / (float)cols.cols;
     warp_cols = (float)__reduce_add_sync(0xffffffffu, cols.count(groups));
     inv_warp_cols = warp_cols > 0.0f ? 1.0f / warp_cols : 0.0f;
     if (warps > 1 && lane == 0) counts[warp] = warp_cols;
+    if (warp == 0) {
+      for (int i = lane; i < 128; i += 32) box[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (lane >= warps) counts[lane] = 0.0f;
+    }
   }
   __device__ __forceinline__ void meet() { asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(32 * warps) : "memory"); }
-  // Sums over the team of what warp_total4 left: the same bits in every thread.
-  __device__ __forceinline__ float4 exchange(float part) {
-    float4 v;
-    if (warps == 1) {
-      v.x = __shfl_sync(0xffffffffu, part, 0);
-      v.y = __shfl_sync(0xffffffffu, part, 8);
-      v.z = __shfl_sync(0xffffffffu, part, 16);
-      v.w = __shfl_sync(0xffffffffu, part, 24);
-      return v;
-    }
-    turn ^= 32;
-    if ((lane & 7) == 0) reinterpret_cast<float*>(&box[turn + warp])[lane >> 3] = part;
-    meet();
-    if (warps <= 4) {
-      v = box[turn];
-      for (int w = 1; w < warps; ++w) {
-        const float4 o = box[turn + w];
-        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
-      }
-      return v;
-    }
-    const float4 o = lane < warps ? box[turn + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    part = warp_total4(o.x, o.y, o.z, o.w, lane);
-    v.x = __shfl_sync(0xffffffffu, part, 0);
-    v.y = __shfl_sync(0xffffffffu, part, 8);
-    v.z = __shfl_sync(0xffffffffu, part, 16);
-    v.w = __shfl_sync(0xffffffffu, part, 24);
-    return v;
+  static __device__ __forceinline__ float4 spread(float part) {
+    return make_float4(__shfl_sync(0xffffffffu, part, 0), __shfl_sync(0xffffffffu, part, 8), __shfl_sync(0xffffffffu, part, 16),
+                       __shfl_sync(0xffffffffu, part, 24));
   }
-  template <int kWarps> __device__ __forceinline__ float4 merged() const {
-    float4 o[kWarps];
-    float n[kWarps], mean = 0.0f, m2 = 0.0f, a = 0.0f, s = 0.0f;
+  // Sums over the team of what warp_total4 left of each row: the same bits in every thread.
+  template <int kRows> __device__ __forceinline__ void exchange(const float (&part)[kRows], float4 (&v)[kRows]) {
+    if (warps == 1) {
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      o[w] = box[turn + w];
-      n[w] = counts[w];
-      mean = fmaf(n[w], o[w].w, mean);
+      for (int r = 0; r < kRows; ++r) v[r] = spread(part[r]);
+      return;
     }
-    mean *= inv_cols;
+    turn ^= 64;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float off = o[w].w - mean;
-      m2 += fmaf(n[w] * off, off, o[w].x);
-      a += o[w].y;
-      s += fmaf(o[w].y, off, o[w].z);
+    for (int r = 0; r < kRows; ++r)
+      if ((lane & 7) == 0) reinterpret_cast<float*>(&box[turn + 32 * r + warp])[lane >> 3] = part[r];
+    meet();
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const float4* at = box + turn + 32 * r;
+      if (warps <= 4) {
+        const float4 o0 = at[0], o1 = at[1], o2 = at[2], o3 = at[3];
+        v[r] = make_float4((o0.x + o1.x) + (o2.x + o3.x), (o0.y + o1.y) + (o2.y + o3.y), (o0.z + o1.z) + (o2.z + o3.z), (o0.w + o1.w) + (o2.w + o3.w));
+      } else {
+        const float4 o = at[lane];
+        v[r] = spread(warp_total4(o.x, o.y, o.z, o.w, lane));
+      }
     }
-    return make_float4(mean, m2, a, s);
   }
   // Each warp's mean of a row with sums around it -- squared deviations m2, and a and the product sum s = sum a (x - mean_w) of another
   // row a -- become the row's: M2 = sum_w m2_w + n_w (mean_w - mean)^2, S = sum_w s_w + a_w (mean_w - mean).  `part` as warp_total4(m2, a, s, .)
-  // leaves it.  Returns (mean, M2, A, S).
-  __device__ __forceinline__ float4 merge(float mean_w, float part) {
+  // leaves it.  Gives (mean, M2, A, S).
+  template <int kRows> __device__ __forceinline__ void merge(const float (&mean_w)[kRows], const float (&part)[kRows], float4 (&v)[kRows]) {
     if (warps == 1) {
-      const float m2 = __shfl_sync(0xffffffffu, part, 0), a = __shfl_sync(0xffffffffu, part, 8), s = __shfl_sync(0xffffffffu, part, 16);
-      return make_float4(mean_w, m2, a, s);
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const float m2 = __shfl_sync(0xffffffffu, part[r], 0), a = __shfl_sync(0xffffffffu, part[r], 8), s = __shfl_sync(0xffffffffu, part[r], 16);
+        v[r] = make_float4(mean_w[r], m2, a, s);
+      }
+      return;
     }
-    turn ^= 32;
-    if ((lane & 7) == 0) reinterpret_cast<float*>(&box[turn + warp])[lane >> 3] = lane == 24 ? mean_w : part;
+    turn ^= 64;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+      if ((lane & 7) == 0) reinterpret_cast<float*>(&box[turn + 32 * r + warp])[lane >> 3] = lane == 24 ? mean_w[r] : part[r];
     meet();
-    if (warps == 2) return merged<2>();
-    if (warps == 3) return merged<3>();
-    if (warps == 4) return merged<4>();
-    const float4 o = lane < warps ? box[turn + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const float n = lane < warps ? counts[lane] : 0.0f;
-    const float mean = warp_total(n * o.w) * inv_cols;
-    const float off = o.w - mean;
-    part = warp_total4(fmaf(n * off, off, o.x), o.y, fmaf(o.y, off, o.z), 0.0f, lane);
-    return make_float4(mean, __shfl_sync(0xffffffffu, part, 0), __shfl_sync(0xffffffffu, part, 8), __shfl_sync(0xffffffffu, part, 16));
+    if (warps <= 4) {
+      const float4 n = *reinterpret_cast<const float4*>(counts);
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const float4* at = box + turn + 32 * r;
+        const float4 o0 = at[0], o1 = at[1], o2 = at[2], o3 = at[3];
+        const float mean = (fmaf(n.x, o0.w, n.y * o1.w) + fmaf(n.z, o2.w, n.w * o3.w)) * inv_cols;
+        const float d0 = o0.w - mean, d1 = o1.w - mean, d2 = o2.w - mean, d3 = o3.w - mean;
+        v[r].x = mean;
+        v[r].y = (fmaf(n.x * d0, d0, o0.x) + fmaf(n.y * d1, d1, o1.x)) + (fmaf(n.z * d2, d2, o2.x) + fmaf(n.w * d3, d3, o3.x));
+        v[r].z = (o0.y + o1.y) + (o2.y + o3.y);
+        v[r].w = (fmaf(o0.y, d0, o0.z) + fmaf(o1.y, d1, o1.z)) + (fmaf(o2.y, d2, o2.z) + fmaf(o3.y, d3, o3.z));
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const float4 o = box[turn + 32 * r + lane];
+        const float n = counts[lane], mean = warp_total(n * o.w) * inv_cols, off = o.w - mean;
+        v[r] = spread(warp_total4(0.0f, fmaf(n * off, off, o.x), o.y, fmaf(o.y, off, o.z), lane));
+        v[r].x = mean;
+      }
+    }
   }
 };
 
@@ -336,7 +340,7 @@ struct Team {
 __device__ __forceinline__ uint32_t team_max_bits(Team& team, uint32_t bits) {
   bits = __reduce_max_sync(0xffffffffu, bits);
   if (team.warps == 1) return bits;
-  team.turn ^= 32;
+  team.turn ^= 64;
   if (team.lane == 0) team.box[team.turn + team.warp].x = __uint_as_float(bits);
   team.meet();
   return __reduce_max_sync(0xffffffffu, team.lane < team.warps ? __float_as_uint(team.box[team.turn + team.lane].x) : 0u);
@@ -359,8 +363,9 @@ __device__ __forceinline__ float2 row_stats(Team& team, const Columns<kVec>& col
   }
   m2 = warp_total(m2);
   if (team.warps == 1) return make_float2(mean_w, rsqrtf(m2 * team.inv_cols + eps));
-  const float4 st = team.merge(mean_w, m2);       // (the other sums' places hold m2 too, and are not looked at)
-  return make_float2(rms ? 0.0f : st.x, rsqrtf(st.y * team.inv_cols + eps));
+  float4 st[1];
+  team.merge<1>({mean_w}, {m2}, st);              // (the other sums' places hold m2 too, and are not looked at)
+  return make_float2(rms ? 0.0f : st[0].x, rsqrtf(st[0].y * team.inv_cols + eps));
 }
 
 // A row in 8-bit integers: q = rint(x min(127 / a, FLT_MAX)) with a = max |x|, scale a / 127.  A row with an infinity or a NaN has scale
