@@ -30,6 +30,7 @@ __global__ void __launch_bounds__(256) souffle_quantise_rows(const T* __restrict
   __shared__ __align__(16) char box[kTeamBox];
   const int teams = blockDim.x / (32 * warps_per_row), warp = threadIdx.x >> 5;
   const int row = blockIdx.x * teams + warp / warps_per_row;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the product may set itself up meanwhile
   if (row >= rows) return;
   const T* from = x + row * x_stride;
   signed char* to = q + row * q_stride;
@@ -44,23 +45,21 @@ __global__ void __launch_bounds__(256) souffle_quantise_rows(const T* __restrict
     quantise_row<kGroups>(team, cols, v, to, scale + row);
     return;
   }
-  uint32_t most = 0;
+  float top = 0.0f;
   const int groups = (cols_n + 256 * warps_per_row - 1) / (256 * warps_per_row);
-  for (int i = 0; i < groups; ++i) {
-    float v[8];
-    unpack8(cols.load(from, i), v);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) most = max(most, abs_bits(v[j]));
-  }
-  most = team_max_bits(team, most);
+  for (int i = 0; i < groups; ++i) top = max_abs8(top, cols.load(from, i));        // (what lies past the row reads as 0)
+  const uint32_t most = team_max_bits(team, __float_as_uint(top) & 0x7fffffffu);
   const RowScale rs = row_scale(most);
   const bool fine = most < 0x7f800000u;
   for (int i = 0; i < groups; ++i) {
-    float v[8];
-    unpack8(cols.load(from, i), v);
+    const uint2 w = fine ? round_s8(cols.load(from, i), rs.inv) : make_uint2(0u, 0u);
+    if (kVec) {
+      if (cols.has(i, 0)) *reinterpret_cast<uint2*>(to + cols.at(i, 0)) = w;
+    } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (cols.has(i, j)) to[cols.at(i, j)] = (signed char)__float2int_rn(fine ? v[j] * rs.inv : 0.0f);
+      for (int j = 0; j < 8; ++j)
+        if (cols.has(i, j)) to[cols.at(i, j)] = (signed char)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
+    }
   }
   if (threadIdx.x % (32 * warps_per_row) == 0) scale[row] = rs.scale;
 }
@@ -76,15 +75,26 @@ __device__ __forceinline__ void store_value(void* p, int dtype, long long i, flo
   else if (dtype == SOUFFLE_F16) static_cast<__half*>(p)[i] = from_f32<__half>(v);
   else static_cast<__nv_bfloat16*>(p)[i] = from_f32<__nv_bfloat16>(v);
 }
-// tanh-form GELU as v * sigmoid(2u), u = sqrt(2 / pi) (v + 0.044715 v^3): one exponential and one division, exact to a few ulp, so
-// that fp32 outputs keep their bits.
-__device__ __forceinline__ float gelu_sigmoid(float v) {
-  const float u = v * fmaf(v * v, 0.044715f * 0.7978845608028654f, 0.7978845608028654f);
-  return __fdividef(v, 1.0f + ex2_fast(-2.885390081777927f * u));
+// tanh-form GELU as v * sigmoid(2u) = v / (1 + e), e = exp(-2u), u = sqrt(2 / pi) (v + 0.044715 v^3), of two values with one reciprocal:
+// 1 / a = b / (a b).  Exact to a few ulp, so that fp32 outputs keep their bits; the functions of the special unit, one exponential and half
+// a reciprocal a value, take as long as the MMAs of an inner dimension of 768.  Below -7.4 the result is under 1e-17: v stops there, which
+// keeps the product of the two below 2^118; a NaN passes.
+__device__ __forceinline__ uint64_t gelu2(uint64_t v) {
+  float2 x = halves(v);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-7.4f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-7.4f));
+  v = pair(x.x, x.y);
+  constexpr float c = -2.885390081777927f * 0.7978845608028654f;       // -2 / ln 2 * sqrt(2 / pi)
+  const float2 z = halves(mul2(v, fma2(mul2(v, v), pair(c * 0.044715f, c * 0.044715f), pair(c, c))));
+  const float a = 1.0f + ex2_fast(z.x), b = 1.0f + ex2_fast(z.y);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
+  return pair(x.x * (r * b), x.y * (r * a));
 }
+__device__ __forceinline__ float gelu1(float v) { return halves(gelu2(pair(v, 0.0f))).x; }
 __device__ __forceinline__ float activate(float v, int act) {
   if (act == SOUFFLE_ACT_RELU) return v < 0.0f ? 0.0f : v;       // a NaN stays one
-  return act == SOUFFLE_ACT_GELU ? gelu_sigmoid(v) : v;
+  return act == SOUFFLE_ACT_GELU ? gelu1(v) : v;
 }
 
 // ---- few tokens --------------------------------------------------------------------------------------------------
@@ -153,24 +163,35 @@ __global__ void __launch_bounds__(32 * kFewWarps) souffle_int8_few(const LinearA
 
 // A pair of CTAs computes tiles of 256 tokens x bn channels with pair MMAs of kind::i8: each CTA loads its own 128 rows of tokens and
 // half of the tile's channels, 128 bytes of the inner dimension at a time, and finds its 128 x bn sums in its own tensor memory.
-// Warp 0 feeds, warp 1 of the pair's leader issues the MMAs, warps 2-9 turn the sums of one tile into outputs while the next
-// tile's are computed in the other half of tensor memory.  Zeros past the matrices' ends come from the copy engine.
-constexpr int kPairThreads = 320, kPairStages = 5, kPairOperand = 128 * 128, kPairEpiWarps = 8, kPairBox = 2048, kPairMaxBn = 256;
+// Warp 0 feeds, warp 1 of the pair's leader issues the MMAs, the others turn the sums of one tile into outputs while the next
+// tile's are computed in the other half of tensor memory, 32 rows x 32 columns at a time and each by itself.  Zeros past the
+// matrices' ends come from the copy engine.
+constexpr int kPairEpiWarps = 16, kPairThreads = 64 + 32 * kPairEpiWarps, kPairStages = 5, kPairOperand = 128 * 128, kPairBox = 2048;
 constexpr unsigned long long kPairTimeoutNs = 2000000000ull;
 struct PairCtl {
   uint64_t full[kPairStages], empty[kPairStages], tmem_full[2], tmem_empty[2];
   WaitCtl wait;
   uint32_t tmem_base;
   int abort;
-  float w_scale[2][kPairMaxBn], bias[2][kPairMaxBn];
+  alignas(16) float w_scale[kPairEpiWarps][64], bias[kPairEpiWarps][64];      // of a warp's chunks
 };
-constexpr int kPairRing = 2 * kPairStages * kPairOperand, kPairBoxes = 2 * kPairEpiWarps * kPairBox;
+constexpr int kPairRing = 2 * kPairStages * kPairOperand, kPairBoxes = kPairEpiWarps * kPairBox;
 constexpr int kPairSmem = kPairRing + kPairBoxes + (int)sizeof(PairCtl) + 1024;      // 1024: the base need not be aligned
 
 struct PairArgs {
-  CUtensorMap x, w, out;
+  CUtensorMap x, w;
   LinearArgs a;
   int bn, tiles_n, tiles, chunks;
+};
+// Where a tile lies, in tiles; the next one of a pair is step_m rows and step_n columns of tiles further (divisions take a warp 150
+// cycles each).
+struct TileAt {
+  int m, n;
+  __device__ __forceinline__ void next(const PairArgs& p, int step_m, int step_n) {
+    m += step_m;
+    n += step_n;
+    if (n >= p.tiles_n) n -= p.tiles_n, ++m;
+  }
 };
 
 // {code, where, cta, 0} of the first wait that ran out since the status was last read
@@ -183,8 +204,19 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, fl
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// kBoxed: the outputs' rows begin on 16-byte boundaries, so that the copy engine can write them.
-template <class T, bool kBoxed>
+// 32 bytes to global memory, which begin on a boundary of 32 or of 16.
+__device__ __forceinline__ void store32(void* to, const uint32_t* w, bool aligned32) {
+  if (aligned32) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+  } else {
+    static_cast<uint4*>(to)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    static_cast<uint4*>(to)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+
+// kWide: the outputs' rows begin on 16-byte boundaries.
+template <class T, bool kWide>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) souffle_int8_pairs(const __grid_constant__ PairArgs p) {
   extern __shared__ uint8_t raw[];
   uint8_t* base = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);       // the same in both CTAs: their windows begin alike
@@ -210,21 +242,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) sou
     fence_mbar_init();
   }
   if (warp == 1) tmem_alloc_pair(smem_u32(&cs.tmem_base), 512);
-  if (warp == 0 && lane < 3) tma_prefetch_desc(lane == 0 ? &p.x : lane == 1 ? &p.w : &p.out);
+  if (warp == 0 && lane < 2) tma_prefetch_desc(lane == 0 ? &p.x : &p.w);
   tc_fence_before_sync();
   __syncthreads();
   cluster_sync_all();                  // the peer's barriers exist before anything arrives on them
   tc_fence_after_sync();
   const uint32_t tmem = cs.tmem_base;
-  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1, step_m = step / p.tiles_n, step_n = step % p.tiles_n;
+  const TileAt first_tile = {first / p.tiles_n, first % p.tiles_n};
+
+  // The rows' quantisation may still be running: their values and scales are not read before it has ended.
+  auto wait_for_rows = [] { asm volatile("griddepcontrol.wait;" ::: "memory"); };
 
   if (warp == 0) {
     if (elect_one()) {
+      wait_for_rows();
       const uint32_t half = (uint32_t)(p.bn >> 1) * 128u;
       uint32_t s = 0, parity = 1;      // a slot that has never been used is empty
       bool ok = true;
-      for (int t = first; ok && t < p.tiles; t += step) {
-        const int m0 = (t / p.tiles_n) * 256 + (int)rank * 128, n0 = (t % p.tiles_n) * p.bn + (int)rank * (p.bn >> 1);
+      TileAt tile = first_tile;
+      for (int t = first; ok && t < p.tiles; t += step, tile.next(p, step_m, step_n)) {
+        const int m0 = tile.m * 256 + (int)rank * 128, n0 = tile.n * p.bn + (int)rank * (p.bn >> 1);
         for (int c = 0; c < p.chunks; ++c) {
           if (!(ok = mbar_wait_hot(smem_u32(&cs.empty[s]), parity, cs.wait, 1))) break;
           const uint32_t full = smem_u32(&cs.full[s]), at = ring + s * 2 * kPairOperand;
@@ -257,79 +295,122 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) sou
       }
     }
   } else {
-    constexpr int kBoxCols = 64 / (int)sizeof(T);
-    const int quarter = warp & 3, part = (warp - 2) >> 2, tid = threadIdx.x - 64;
-    uint8_t* box = boxes + (warp - 2) * 2 * kPairBox;
-    uint32_t buf = 0, parity = 0, which = 0;
-    for (int t = first; t < p.tiles; t += step) {
-      const int m0 = (t / p.tiles_n) * 256 + (int)rank * 128 + quarter * 32, n0 = (t % p.tiles_n) * p.bn;
-      if (tid < p.bn) {
-        const int n = n0 + tid;
-        cs.w_scale[buf][tid] = n < a.cols ? a.w_scale[n] : 0.0f;
-        cs.bias[buf][tid] = a.bias && n < a.cols ? to_f32(static_cast<const T*>(a.bias)[n]) : 0.0f;
+    constexpr int kBoxCols = 64 / (int)sizeof(T), kStep = 32 * kPairEpiWarps / 4;       // four lane quarters
+    const int quarter = warp & 3, own = warp - 2, part = own >> 2;
+    const bool aligned32 = (((uintptr_t)a.out | (uintptr_t)(a.out_stride * (long long)sizeof(T))) & 31u) == 0;
+    uint8_t* at = boxes + own * kPairBox;
+    uint32_t buf = 0, parity = 0;
+    // What a tile needs beside its sums is read a tile ahead (a read takes a thousand cycles beside the copies): the scales and biases of
+    // this warp's chunks of 32 columns, one a lane, and the lane's row's scale.
+    constexpr int kChunks = 256 / kStep;
+    float next_w[kChunks], next_x;
+    T next_b[kChunks];                 // (as it is stored: its conversion would wait for it)
+    auto look_up = [&](const TileAt& to) {
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int c = 32 * part + i * kStep + lane, n = to.n * p.bn + c;
+        const bool there = c < p.bn && n < a.cols;
+        next_w[i] = there ? a.w_scale[n] : 0.0f;
+        next_b[i] = there && a.bias ? static_cast<const T*>(a.bias)[n] : from_f32<T>(0.0f);
       }
-      const float xs = m0 + lane < a.rows ? a.x_scale[m0 + lane] : 0.0f;
-      named_barrier_sync(1, 32 * kPairEpiWarps);
-      const bool ok = mbar_wait_warp(smem_u32(&cs.tmem_full[buf]), parity, cs.wait, 4, lane);
-      if (ok) {                        // (all warps go through the tiles and meet at their barriers, given up or not)
+    };
+    auto look_up_row = [&](const TileAt& to) {
+      const int m = to.m * 256 + (int)rank * 128 + quarter * 32 + lane;
+      next_x = m < a.rows ? a.x_scale[m] : 0.0f;
+    };
+    TileAt tile = first_tile;
+    look_up(tile);
+    wait_for_rows();
+    look_up_row(tile);
+    for (int t = first; t < p.tiles; t += step) {
+      const int m0 = tile.m * 256 + (int)rank * 128 + quarter * 32, n0 = tile.n * p.bn;
+      const uint64_t xs = pair(next_x, next_x);
+      __syncwarp();                    // everybody has read the last tile's scales
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        cs.w_scale[own][32 * i + lane] = next_w[i];
+        cs.bias[own][32 * i + lane] = to_f32(next_b[i]);
+      }
+      tile.next(p, step_m, step_n);
+      if (t + step < p.tiles) {
+        look_up(tile);
+        look_up_row(tile);
+      }
+      __syncwarp();
+      if (mbar_wait_hot(smem_u32(&cs.tmem_full[buf]), parity, cs.wait, 4)) {       // (all go through the tiles, given up or not)
+        __syncwarp();
         tc_fence_after_sync();
-        for (int c0 = 32 * part; c0 < p.bn; c0 += 64) {
+        const uint32_t sums = tmem + ((uint32_t)(quarter * 32) << 16) + buf * 256;
+        const int ends = p.bn < a.cols - n0 ? p.bn : a.cols - n0;
+#pragma unroll
+        for (int chunk = 0; chunk < kChunks; ++chunk) {
+          const int c0 = 32 * part + chunk * kStep;
+          if (c0 >= ends) break;
           uint32_t r[32];
-          tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + buf * 256 + c0, r);
+          tmem_ld32(sums + c0, r);
+          uint64_t v[16];
           tmem_ld_wait(r);
-          if (n0 + c0 >= a.cols) continue;
-          float v[32];
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 w = *reinterpret_cast<const float4*>(&cs.w_scale[buf][c0 + i]), b = *reinterpret_cast<const float4*>(&cs.bias[buf][c0 + i]);
-            v[i] = fmaf((float)(int)r[i] * xs, w.x, b.x);
-            v[i + 1] = fmaf((float)(int)r[i + 1] * xs, w.y, b.y);
-            v[i + 2] = fmaf((float)(int)r[i + 2] * xs, w.z, b.z);
-            v[i + 3] = fmaf((float)(int)r[i + 3] * xs, w.w, b.w);
+          for (int i = 0; i < 16; ++i) v[i] = mul2(pair((float)(int)r[2 * i], (float)(int)r[2 * i + 1]), xs);
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(&cs.w_scale[own][32 * chunk + 2 * i]), b = *reinterpret_cast<const ulonglong2*>(&cs.bias[own][32 * chunk + 2 * i]);
+            v[i] = fma2(v[i], w.x, b.x);
+            v[i + 1] = fma2(v[i + 1], w.y, b.y);
           }
-          if (a.act == SOUFFLE_ACT_RELU) {
+          if (a.act == SOUFFLE_ACT_GELU) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
-          } else if (a.act == SOUFFLE_ACT_GELU) {
+            for (int i = 0; i < 16; ++i) v[i] = gelu2(v[i]);
+          } else if (a.act == SOUFFLE_ACT_RELU) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = gelu_sigmoid(v[i]);
+            for (int i = 0; i < 16; ++i) {
+              const float2 x = halves(v[i]);
+              v[i] = pair(x.x < 0.0f ? 0.0f : x.x, x.y < 0.0f ? 0.0f : x.y);
+            }
           }
           uint32_t words[8 * sizeof(T)];
-          if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) words[i] = __float_as_uint(v[i]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) words[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
-          }
-#pragma unroll
-          for (int b = 0; b < 32 / kBoxCols; ++b) {
-            uint8_t* at = box + which * kPairBox;
-            if (kBoxed) {
-              if (lane == 0) bulk_wait_group_read<1>();        // the box's last copy has read it
-              __syncwarp();
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)                          // the layout of a 64B-swizzled box
-              *reinterpret_cast<uint4*>(at + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
-                  make_uint4(words[16 * b + 4 * i], words[16 * b + 4 * i + 1], words[16 * b + 4 * i + 2], words[16 * b + 4 * i + 3]);
-            if (kBoxed) {
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) {
-                if (n0 + c0 + b * kBoxCols < a.cols && m0 < a.rows) tma_store_2d(&p.out, smem_u32(at), n0 + c0 + b * kBoxCols, m0);
-                bulk_commit_group();
-              }
+          for (int i = 0; i < 16; ++i) {
+            const float2 x = halves(v[i]);
+            if constexpr (sizeof(T) == 4) {
+              words[2 * i] = __float_as_uint(x.x);
+              words[2 * i + 1] = __float_as_uint(x.y);
             } else {
+              words[i] = pack2<T>(x.x, x.y);
+            }
+          }
+          if (kWide) {
+            // Straight from the registers, 32 bytes a lane and store, whole sectors of the lane's row.  Shared memory's bandwidth is what
+            // this kernel runs at (a tile of 256 x 192: copies in 168 KB, MMAs read 240 KB), so outputs do not pass it again: through it
+            // 8192 x 768 x 3072 took 25.0 us, 32.6 with GELU.
+            T* out = static_cast<T*>(a.out) + (m0 + lane) * a.out_stride + n0 + c0;
+            if (m0 + lane < a.rows) {
+              if (c0 + 32 <= a.cols - n0) {
+#pragma unroll
+                for (int i = 0; i < (int)sizeof(T); ++i) store32(out + i * (32 / (int)sizeof(T)), &words[8 * i], aligned32);
+              } else {
+                const T* each = reinterpret_cast<const T*>(words);
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (c0 + i < a.cols - n0) out[i] = each[i];
+              }
+            }
+          } else {
+            // rows begin anywhere: through shared memory, 32 rows x 64 bytes at a time, so that a store's lanes write neighbouring elements
+#pragma unroll
+            for (int b = 0; b < 32 / kBoxCols; ++b) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<uint4*>(at + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
+                    make_uint4(words[16 * b + 4 * i], words[16 * b + 4 * i + 1], words[16 * b + 4 * i + 2], words[16 * b + 4 * i + 3]);
               __syncwarp();
-              const int c = lane % kBoxCols, n = n0 + c0 + b * kBoxCols + c;
+              const int n = n0 + c0 + b * kBoxCols, c = lane % kBoxCols;
               for (int row = lane / kBoxCols; row < 32; row += 32 / kBoxCols) {
                 const T value = *reinterpret_cast<const T*>(at + row * 64 + ((((c * (int)sizeof(T)) >> 4) ^ ((row >> 1) & 3)) << 4) + ((c * (int)sizeof(T)) & 15));
-                if (n < a.cols && m0 + row < a.rows) static_cast<T*>(a.out)[(m0 + row) * a.out_stride + n] = value;
+                if (n + c < a.cols && m0 + row < a.rows) static_cast<T*>(a.out)[(m0 + row) * a.out_stride + n + c] = value;
               }
               __syncwarp();
             }
-            which ^= 1;
           }
         }
         tc_fence_before_sync();
@@ -338,7 +419,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) sou
       }
       if (buf ^= 1, buf == 0) parity ^= 1;
     }
-    if (kBoxed && lane == 0) bulk_wait_group_all();
   }
 
   __syncthreads();
@@ -367,7 +447,7 @@ static int quantise_launch(const T* x, long long x_stride, int rows, int cols, s
   const int threads = warps == 1 ? 128 : 32 * warps, teams = threads / (32 * warps), grid = (rows + teams - 1) / teams;
   const int groups = (groups8 + 32 * warps - 1) / (32 * warps);
   auto go = [&](auto fn) { fn<<<grid, threads, 0, st>>>(x, x_stride, rows, cols, q, q_stride, scale, warps); };
-  if (vec) groups <= 1 ? go(souffle_quantise_rows<T, true, 1>) : groups == 2 ? go(souffle_quantise_rows<T, true, 2>) : go(souffle_quantise_rows<T, true, 4>);
+  if (vec) groups <= 1 ? go(souffle_quantise_rows<T, true, 1>) : groups == 2 ? go(souffle_quantise_rows<T, true, 2>) : groups == 3 ? go(souffle_quantise_rows<T, true, 3>) : go(souffle_quantise_rows<T, true, 4>);
   else groups <= 1 ? go(souffle_quantise_rows<T, false, 1>) : groups == 2 ? go(souffle_quantise_rows<T, false, 2>) : go(souffle_quantise_rows<T, false, 4>);
   SF_CUDA(cudaGetLastError());
   return SOUFFLE_OK;
@@ -379,13 +459,13 @@ static int quantise(const void* x, int dtype, long long x_stride, int rows, int 
 }
 static long long padded16(long long n) { return (n + 15) / 16 * 16; }
 
-static int make_map(CUtensorMap* m, CUtensorMapDataType type, const void* p, uint64_t rows, uint64_t cols, uint64_t pitch_bytes, uint32_t box_cols,
-                    uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+// A map of 8-bit rows for tiles of box_rows rows x 128 bytes.
+static int make_map(CUtensorMap* m, const void* p, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(SOUFFLE_CUDA_ERROR, "cuTensorMapEncodeTiled is not available from the driver");
-  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch_bytes};
-  const cuuint32_t box[2] = {box_cols, box_rows}, one[2] = {1, 1};
-  const CUresult r = fn(m, type, 2, const_cast<void*>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch};
+  const cuuint32_t box[2] = {128, box_rows}, one[2] = {1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? SOUFFLE_OK : fail(SOUFFLE_CUDA_ERROR, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
 }
@@ -405,7 +485,7 @@ static int choose_bn(int rows, int inner, int cols, int act, int pairs) {
 }
 
 template <class T>
-static int pairs_launch(const LinearArgs& a, int sms, cudaStream_t st) {
+static int pairs_launch(const LinearArgs& a, bool behind_quantisation, int sms, int dev, cudaStream_t st) {
   PairArgs p;
   p.a = a;
   p.bn = choose_bn(a.rows, a.inner, a.cols, a.act, sms / 2);
@@ -415,21 +495,26 @@ static int pairs_launch(const LinearArgs& a, int sms, cudaStream_t st) {
   if (tiles > (1 << 30)) return fail(SOUFFLE_BAD_SHAPE, "8-bit product of %d x %d: too many tiles", a.rows, a.cols);
   p.tiles = (int)tiles;
   int rc;
-  if ((rc = make_map(&p.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.x, a.rows, a.inner, a.x_stride, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B)) ||
-      (rc = make_map(&p.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w, a.cols, a.inner, a.w_stride, 128, p.bn / 2, CU_TENSOR_MAP_SWIZZLE_128B)))
-    return rc;
-  const bool boxed = ((uintptr_t)a.out & 15u) == 0 && (a.out_stride * (long long)sizeof(T)) % 16 == 0;
-  if (boxed) {
-    const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
-    if ((rc = make_map(&p.out, type, a.out, a.rows, a.cols, a.out_stride * sizeof(T), 64 / sizeof(T), 32, CU_TENSOR_MAP_SWIZZLE_64B))) return rc;
-  } else {
-    p.out = p.x;                       // a map that exists, for the prefetch
+  if ((rc = make_map(&p.x, a.x, a.rows, a.inner, a.x_stride, 128)) || (rc = make_map(&p.w, a.w, a.cols, a.inner, a.w_stride, p.bn / 2))) return rc;
+  const bool wide = ((uintptr_t)a.out & 15u) == 0 && (a.out_stride * (long long)sizeof(T)) % 16 == 0;
+  auto fn = wide ? souffle_int8_pairs<T, true> : souffle_int8_pairs<T, false>;
+  static bool ready[2][kMaxDevices];
+  if (!ready[wide][dev]) {
+    SF_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+    ready[wide][dev] = true;
   }
-  auto fn = boxed ? souffle_int8_pairs<T, true> : souffle_int8_pairs<T, false>;
-  SF_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
-  const int pairs = p.tiles < sms / 2 ? p.tiles : sms / 2;
-  fn<<<2 * pairs, kPairThreads, kPairSmem, st>>>(p);
-  SF_CUDA(cudaGetLastError());
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(2 * (p.tiles < sms / 2 ? p.tiles : sms / 2));
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = behind_quantisation ? 1 : 0;
+  SF_CUDA(cudaLaunchKernelEx(&cfg, fn, p));
   return SOUFFLE_OK;
 }
 
@@ -478,7 +563,7 @@ int souffle_int8_linear_forward(const SouffleInt8Linear* call, souffle_stream_t 
     return fail(SOUFFLE_BAD_POINTER, "null or misaligned pointer");
   const size_t need = souffle_int8_linear_workspace_bytes(d.rows, d.inner, d.x_dtype);
   if (need && (!aligned16(d.workspace) || d.workspace_bytes < need)) return fail(SOUFFLE_BAD_POINTER, "workspace is null, misaligned or smaller than souffle_int8_linear_workspace_bytes()");
-  int sms, rc = current_sms(&sms);
+  int sms, dev, rc = current_sms(&sms, &dev);
   if (rc) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   LinearArgs a;
@@ -492,8 +577,8 @@ int souffle_int8_linear_forward(const SouffleInt8Linear* call, souffle_stream_t 
     a.x = q; a.x_scale = scale; a.x_stride = padded16(d.inner);
   }
   if (d.rows > kFewRows) {
-    if (d.out_dtype == SOUFFLE_F32) return pairs_launch<float>(a, sms, st);
-    return d.out_dtype == SOUFFLE_F16 ? pairs_launch<__half>(a, sms, st) : pairs_launch<__nv_bfloat16>(a, sms, st);
+    if (d.out_dtype == SOUFFLE_F32) return pairs_launch<float>(a, !given, sms, dev, st);
+    return d.out_dtype == SOUFFLE_F16 ? pairs_launch<__half>(a, !given, sms, dev, st) : pairs_launch<__nv_bfloat16>(a, !given, sms, dev, st);
   }
   souffle_int8_few<2><<<dim3((d.cols + 15) / 16, (d.rows + 15) / 16), 32 * kFewWarps, 0, st>>>(a);
   SF_CUDA(cudaGetLastError());

@@ -377,37 +377,62 @@ __device__ __forceinline__ RowScale row_scale(uint32_t max_bits) {
   const float a = __uint_as_float(max_bits);
   return {fminf(127.0f / a, 3.402823466e38f), a / 127.0f};
 }
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-// four values, in the order of the bytes
-__device__ __forceinline__ uint32_t pack_s8(float a, float b, float c, float d) {
-  return (uint32_t)(__float2int_rn(a) & 255) | (uint32_t)(__float2int_rn(b) & 255) << 8 | (uint32_t)(__float2int_rn(c) & 255) << 16 |
-         (uint32_t)(__float2int_rn(d)) << 24;
+// max(m, |v|) that keeps a NaN
+__device__ __forceinline__ float max_abs(float m, float v) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(v)));
+  return r;
+}
+__device__ __forceinline__ float max_abs8(float m, const F8& x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = halves(x.p[i]);
+    m = max_abs(max_abs(m, v.x), v.y);
+  }
+  return m;
+}
+// The eight values times `inv`, rounded half to even, as bytes: a sum with 1.5 * 2^23 holds the integer in its lowest bits, two's
+// complement included (conversions to integers run at a quarter of the rate).
+__device__ __forceinline__ uint2 round_s8(const F8& x, float inv) {
+  float2 v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 h = halves(x.p[i]);         // (one by one: a product and a sum of pairs would become one operation, with one rounding)
+    v[i] = halves(add2(pair(__fmul_rn(h.x, inv), __fmul_rn(h.y, inv)), pair(12582912.0f, 12582912.0f)));
+  }
+  const float2 a = v[0], b = v[1], c = v[2], d = v[3];
+  auto four = [](float2 p, float2 q) {
+    return __byte_perm(__byte_perm(__float_as_uint(p.x), __float_as_uint(p.y), 0x0040), __byte_perm(__float_as_uint(q.x), __float_as_uint(q.y), 0x0040), 0x5410);
+  };
+  return make_uint2(four(a, b), four(c, d));
 }
 template <int kGroups, class C>
 __device__ __forceinline__ void quantise_row(Team& team, const C& cols, const F8 (&x)[kGroups], signed char* q, float* scale) {
-  uint32_t most = 0;
-  float v[8];
+  float top = 0.0f;
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
-    unpack8(x[i], v);
+    if (C::kVec) {
+      if (cols.has(i, 0)) top = max_abs8(top, x[i]);
+    } else {
+      float v[8];
+      unpack8(x[i], v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (cols.has(i, j)) most = max(most, abs_bits(v[j]));
+      for (int j = 0; j < 8; ++j)
+        if (cols.has(i, j)) top = max_abs(top, v[j]);
+    }
   }
-  most = team_max_bits(team, most);
+  const uint32_t most = team_max_bits(team, __float_as_uint(top) & 0x7fffffffu);
   const RowScale rs = row_scale(most);
   const bool fine = most < 0x7f800000u;      // 0 * inf is no number
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
-    unpack8(x[i], v);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = fine ? v[j] * rs.inv : 0.0f;
+    const uint2 w = fine ? round_s8(x[i], rs.inv) : make_uint2(0u, 0u);
     if (C::kVec) {
-      if (cols.has(i, 0)) *reinterpret_cast<uint2*>(q + cols.at(i, 0)) = make_uint2(pack_s8(v[0], v[1], v[2], v[3]), pack_s8(v[4], v[5], v[6], v[7]));
+      if (cols.has(i, 0)) *reinterpret_cast<uint2*>(q + cols.at(i, 0)) = w;
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (cols.has(i, j)) q[cols.at(i, j)] = (signed char)__float2int_rn(v[j]);
+        if (cols.has(i, j)) q[cols.at(i, j)] = (signed char)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
     }
   }
   if (team.warp == 0 && team.lane == 0) *scale = rs.scale;
