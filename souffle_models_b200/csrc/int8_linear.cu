@@ -166,22 +166,23 @@ __global__ void __launch_bounds__(32 * kFewWarps) souffle_int8_few(const LinearA
 // Warp 0 feeds, warp 1 of the pair's leader issues the MMAs, the others turn the sums of one tile into outputs while the next
 // tile's are computed in the other half of tensor memory, 32 rows x 32 columns at a time and each by itself.  Zeros past the
 // matrices' ends come from the copy engine.
-constexpr int kPairEpiWarps = 16, kPairThreads = 64 + 32 * kPairEpiWarps, kPairStages = 5, kPairOperand = 128 * 128, kPairBox = 2048;
+constexpr int kPairMaxStages = 8, kPairOperand = 128 * 128, kPairBox = 4096, kParts = 2 /* epilogue warps a lane quarter */, kPairThreads = 64 + 128 * kParts;
 constexpr unsigned long long kPairTimeoutNs = 2000000000ull;
 struct PairCtl {
-  uint64_t full[kPairStages], empty[kPairStages], tmem_full[2], tmem_empty[2];
+  uint64_t full[kPairMaxStages], empty[kPairMaxStages], tmem_full[2], tmem_empty[2];
   WaitCtl wait;
   uint32_t tmem_base;
   int abort;
-  alignas(16) float w_scale[kPairEpiWarps][64], bias[kPairEpiWarps][64];      // of a warp's chunks
+  alignas(16) float w_scale[1024], bias[1024];      // of each epilogue warp's columns
 };
-constexpr int kPairRing = 2 * kPairStages * kPairOperand, kPairBoxes = kPairEpiWarps * kPairBox;
-constexpr int kPairSmem = kPairRing + kPairBoxes + (int)sizeof(PairCtl) + 1024;      // 1024: the base need not be aligned
+// Shared memory: the ring, a box for each epilogue warp, PairCtl, and room to begin on a boundary of 1024 bytes.
+constexpr int kPairMostSmem = 227 * 1024, kPairFixedSmem = 4 * kParts * kPairBox + (int)sizeof(PairCtl) + 1024;
 
 struct PairArgs {
-  CUtensorMap x, w;
+  CUtensorMap x, w, out;
   LinearArgs a;
   int bn, tiles_n, tiles, chunks;
+  int stages, slot_bytes;              // of the ring
 };
 // Where a tile lies, in tiles; the next one of a pair is step_m rows and step_n columns of tiles further (divisions take a warp 150
 // cycles each).
@@ -204,36 +205,25 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, fl
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// 32 bytes to global memory, which begin on a boundary of 32 or of 16.
-__device__ __forceinline__ void store32(void* to, const uint32_t* w, bool aligned32) {
-  if (aligned32) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                 ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
-  } else {
-    static_cast<uint4*>(to)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-    static_cast<uint4*>(to)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-  }
-}
-
 // kWide: the outputs' rows begin on 16-byte boundaries.
 template <class T, bool kWide>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) souffle_int8_pairs(const __grid_constant__ PairArgs p) {
   extern __shared__ uint8_t raw[];
   uint8_t* base = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);       // the same in both CTAs: their windows begin alike
   const uint32_t ring = smem_u32(base);
-  uint8_t* boxes = base + kPairRing;
-  PairCtl& cs = *reinterpret_cast<PairCtl*>(boxes + kPairBoxes);
+  uint8_t* boxes = base + p.stages * p.slot_bytes;
+  PairCtl& cs = *reinterpret_cast<PairCtl*>(boxes + 4 * kParts * kPairBox);
   const LinearArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_cta_rank();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kPairStages; ++i) {
+    for (int i = 0; i < p.stages; ++i) {
       mbar_init(smem_u32(&cs.full[i]), 1);
       mbar_init(smem_u32(&cs.empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&cs.tmem_full[i]), 1);
-      mbar_init(smem_u32(&cs.tmem_empty[i]), 2 * kPairEpiWarps);
+      mbar_init(smem_u32(&cs.tmem_empty[i]), 2 * 4 * kParts);
     }
     cs.abort = 0;
     cs.wait.abort_smem = &cs.abort;
@@ -242,7 +232,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) sou
     fence_mbar_init();
   }
   if (warp == 1) tmem_alloc_pair(smem_u32(&cs.tmem_base), 512);
-  if (warp == 0 && lane < 2) tma_prefetch_desc(lane == 0 ? &p.x : &p.w);
+  if (warp == 0 && lane < 2 + kWide) tma_prefetch_desc(lane == 0 ? &p.x : lane == 1 ? &p.w : &p.out);
   tc_fence_before_sync();
   __syncthreads();
   cluster_sync_all();                  // the peer's barriers exist before anything arrives on them
@@ -265,12 +255,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) sou
         const int m0 = tile.m * 256 + (int)rank * 128, n0 = tile.n * p.bn + (int)rank * (p.bn >> 1);
         for (int c = 0; c < p.chunks; ++c) {
           if (!(ok = mbar_wait_hot(smem_u32(&cs.empty[s]), parity, cs.wait, 1))) break;
-          const uint32_t full = smem_u32(&cs.full[s]), at = ring + s * 2 * kPairOperand;
+          const uint32_t full = smem_u32(&cs.full[s]), at = ring + s * p.slot_bytes;
           if (rank == 0) mbar_expect_tx(full, 2 * (kPairOperand + half));
           const uint32_t leader = map_shared_rank(full, 0);
           tma_load_2d_pair(at, &p.x, leader, c * 128, m0);
           tma_load_2d_pair(at + kPairOperand, &p.w, leader, c * 128, n0);
-          if (++s == kPairStages) s = 0, parity ^= 1;
+          if (++s == (uint32_t)p.stages) s = 0, parity ^= 1;
         }
       }
     }
@@ -285,30 +275,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) sou
         for (int c = 0; c < p.chunks; ++c) {
           if (!(ok = mbar_wait_hot(smem_u32(&cs.full[s]), parity, cs.wait, 3))) break;
           tc_fence_after_sync();
-          const uint32_t at = ring + s * 2 * kPairOperand;
+          const uint32_t at = ring + s * p.slot_bytes;
           umma_i8_k128_pair(tmem + buf * 256, umma_desc_lo(at, 16), umma_desc_lo(at + kPairOperand, 16), idesc, c != 0);
           umma_commit_pair(smem_u32(&cs.empty[s]));
-          if (++s == kPairStages) s = 0, parity ^= 1;
+          if (++s == (uint32_t)p.stages) s = 0, parity ^= 1;
         }
         if (ok) umma_commit_pair(smem_u32(&cs.tmem_full[buf]));
         if (buf ^= 1, buf == 0) free_parity ^= 1;
       }
     }
   } else {
-    constexpr int kBoxCols = 64 / (int)sizeof(T), kStep = 32 * kPairEpiWarps / 4;       // four lane quarters
+    constexpr int kBoxCols = 128 / (int)sizeof(T);      // a box: 32 rows x 128 bytes
     const int quarter = warp & 3, own = warp - 2, part = own >> 2;
-    const bool aligned32 = (((uintptr_t)a.out | (uintptr_t)(a.out_stride * (long long)sizeof(T))) & 31u) == 0;
     uint8_t* at = boxes + own * kPairBox;
     uint32_t buf = 0, parity = 0;
     // What a tile needs beside its sums is read a tile ahead (a read takes a thousand cycles beside the copies): the scales and biases of
     // this warp's chunks of 32 columns, one a lane, and the lane's row's scale.
-    constexpr int kChunks = 256 / kStep;
+    constexpr int kChunks = 8 / kParts;       // of 32 columns: pieces of 64 are dealt out to the warps of a lane quarter
+    const int mine = 32 * kChunks * own;
+    auto chunk_at = [&](int i) { return 64 * (part + (i >> 1) * kParts) + 32 * (i & 1); };
     float next_w[kChunks], next_x;
     T next_b[kChunks];                 // (as it is stored: its conversion would wait for it)
     auto look_up = [&](const TileAt& to) {
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
-        const int c = 32 * part + i * kStep + lane, n = to.n * p.bn + c;
+        const int c = chunk_at(i) + lane, n = to.n * p.bn + c;
         const bool there = c < p.bn && n < a.cols;
         next_w[i] = there ? a.w_scale[n] : 0.0f;
         next_b[i] = there && a.bias ? static_cast<const T*>(a.bias)[n] : from_f32<T>(0.0f);
@@ -328,8 +319,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) sou
       __syncwarp();                    // everybody has read the last tile's scales
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
-        cs.w_scale[own][32 * i + lane] = next_w[i];
-        cs.bias[own][32 * i + lane] = to_f32(next_b[i]);
+        cs.w_scale[mine + 32 * i + lane] = next_w[i];
+        cs.bias[mine + 32 * i + lane] = to_f32(next_b[i]);
       }
       tile.next(p, step_m, step_n);
       if (t + step < p.tiles) {
@@ -344,7 +335,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) sou
         const int ends = p.bn < a.cols - n0 ? p.bn : a.cols - n0;
 #pragma unroll
         for (int chunk = 0; chunk < kChunks; ++chunk) {
-          const int c0 = 32 * part + chunk * kStep;
+          const int c0 = chunk_at(chunk), second = chunk & 1;
           if (c0 >= ends) break;
           uint32_t r[32];
           tmem_ld32(sums + c0, r);
@@ -354,7 +345,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) sou
           for (int i = 0; i < 16; ++i) v[i] = mul2(pair((float)(int)r[2 * i], (float)(int)r[2 * i + 1]), xs);
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
-            const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(&cs.w_scale[own][32 * chunk + 2 * i]), b = *reinterpret_cast<const ulonglong2*>(&cs.bias[own][32 * chunk + 2 * i]);
+            const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(&cs.w_scale[mine + 32 * chunk + 2 * i]), b = *reinterpret_cast<const ulonglong2*>(&cs.bias[mine + 32 * chunk + 2 * i]);
             v[i] = fma2(v[i], w.x, b.x);
             v[i + 1] = fma2(v[i + 1], w.y, b.y);
           }
@@ -379,38 +370,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) sou
               words[i] = pack2<T>(x.x, x.y);
             }
           }
+          // Outputs leave through a box of 32 rows x 128 bytes, in the layout of a 128B-swizzled one, so that they reach L2 as whole lines:
+          // of 32 bytes a lane, straight from the registers, 8192 x 768 x 3072 took 22.5 us, 14.6 without its stores.
+          const int first_slot = sizeof(T) == 4 ? 0 : 4 * second;        // of a row's eight 16-byte slots
+          if (first_slot == 0) {
+            if (kWide && lane == 0) bulk_wait_group_read<0>();          // the last copy has read the box
+            __syncwarp();
+          }
+#pragma unroll
+          for (int i = 0; i < (int)(2 * sizeof(T)); ++i)
+            *reinterpret_cast<uint4*>(at + lane * 128 + (((first_slot + i) ^ (lane & 7)) << 4)) = make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
+          const bool full = sizeof(T) == 4 || second || c0 + 32 >= ends;
+          if (!full) continue;
+          const int n = n0 + c0 - (sizeof(T) == 4 ? 0 : 32 * second);
           if (kWide) {
-            // Straight from the registers, 32 bytes a lane and store, whole sectors of the lane's row.  Shared memory's bandwidth is what
-            // this kernel runs at (a tile of 256 x 192: copies in 168 KB, MMAs read 240 KB), so outputs do not pass it again: through it
-            // 8192 x 768 x 3072 took 25.0 us, 32.6 with GELU.
-            T* out = static_cast<T*>(a.out) + (m0 + lane) * a.out_stride + n0 + c0;
-            if (m0 + lane < a.rows) {
-              if (c0 + 32 <= a.cols - n0) {
-#pragma unroll
-                for (int i = 0; i < (int)sizeof(T); ++i) store32(out + i * (32 / (int)sizeof(T)), &words[8 * i], aligned32);
-              } else {
-                const T* each = reinterpret_cast<const T*>(words);
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (c0 + i < a.cols - n0) out[i] = each[i];
-              }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && m0 < a.rows) {
+              tma_store_2d(&p.out, smem_u32(at), n, m0);
+              bulk_commit_group();
             }
-          } else {
-            // rows begin anywhere: through shared memory, 32 rows x 64 bytes at a time, so that a store's lanes write neighbouring elements
-#pragma unroll
-            for (int b = 0; b < 32 / kBoxCols; ++b) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<uint4*>(at + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
-                    make_uint4(words[16 * b + 4 * i], words[16 * b + 4 * i + 1], words[16 * b + 4 * i + 2], words[16 * b + 4 * i + 3]);
-              __syncwarp();
-              const int n = n0 + c0 + b * kBoxCols, c = lane % kBoxCols;
-              for (int row = lane / kBoxCols; row < 32; row += 32 / kBoxCols) {
-                const T value = *reinterpret_cast<const T*>(at + row * 64 + ((((c * (int)sizeof(T)) >> 4) ^ ((row >> 1) & 3)) << 4) + ((c * (int)sizeof(T)) & 15));
-                if (n + c < a.cols && m0 + row < a.rows) static_cast<T*>(a.out)[(m0 + row) * a.out_stride + n + c] = value;
+          } else {                     // rows begin anywhere: the lanes write neighbouring elements
+            __syncwarp();
+            const int held = ends + n0 - n < kBoxCols ? ends + n0 - n : kBoxCols;
+            for (int c = lane; c < held; c += 32)
+              for (int row = 0; row < 32; ++row) {
+                if (m0 + row >= a.rows) break;
+                const int byte = c * (int)sizeof(T);
+                static_cast<T*>(a.out)[(m0 + row) * a.out_stride + n + c] = *reinterpret_cast<const T*>(at + row * 128 + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15));
               }
-              __syncwarp();
-            }
+            __syncwarp();
           }
         }
         tc_fence_before_sync();
@@ -419,6 +408,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) sou
       }
       if (buf ^= 1, buf == 0) parity ^= 1;
     }
+    if (kWide && lane == 0) bulk_wait_group_all();
   }
 
   __syncthreads();
@@ -459,27 +449,30 @@ static int quantise(const void* x, int dtype, long long x_stride, int rows, int 
 }
 static long long padded16(long long n) { return (n + 15) / 16 * 16; }
 
-// A map of 8-bit rows for tiles of box_rows rows x 128 bytes.
-static int make_map(CUtensorMap* m, const void* p, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t box_rows) {
+// A map of rows for boxes of box_rows rows x 128 bytes, 128B-swizzled; `pitch` in bytes.
+static int make_map(CUtensorMap* m, CUtensorMapDataType type, uint32_t size, const void* p, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(SOUFFLE_CUDA_ERROR, "cuTensorMapEncodeTiled is not available from the driver");
   const cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch};
-  const cuuint32_t box[2] = {128, box_rows}, one[2] = {1, 1};
-  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  const cuuint32_t box[2] = {128 / size, box_rows}, one[2] = {1, 1};
+  const CUresult r = fn(m, type, 2, const_cast<void*>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? SOUFFLE_OK : fail(SOUFFLE_CUDA_ERROR, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
 }
 
-// The tile width that takes the fewest cycles: whole tiles dealt out to the pairs, each bound by its MMAs (bn / 2 cycles a step of
-// 32, 51 at least) or by its epilogue, the last one's epilogue behind everything.
+// The tile width that takes the fewest cycles by what was measured: whole tiles dealt out to the pairs, each bound by its MMAs (2 bn cycles
+// a step of 128), by its operands' way from L2 (52 bytes a cycle and CTA) or by its epilogue (pieces of 64 columns, two at a time), the last
+// one's epilogue behind everything.  8192 x 768 x 3072 with GELU: 256 29.3 us, 192 27.9, 128 31.6; 8192 x 256 x 1024: 11.4, 12.9, 12.4;
+// 8192 x 3072 x 768 without: 21.7, 18.4, 21.3; 1571 x 1024 x 1024 fp32: 9.1, 8.3, 6.9.
 static int choose_bn(int rows, int inner, int cols, int act, int pairs) {
   int best = 256;
   double least = 1e30;
   for (int bn = 256; bn >= 64; bn -= 64) {
     const long long tiles = ((rows + 255) / 256) * (long long)((cols + bn - 1) / bn), waves = (tiles + pairs - 1) / pairs;
-    const double loop = ((inner + 127) / 128) * 4.0 * (bn / 2 > 51 ? bn / 2 : 51), epi = bn * (act == SOUFFLE_ACT_GELU ? 16.0 : 8.0);
+    const double step = (kPairOperand + 64 * bn) / 52.0, loop = (inner + 127) / 128 * (step > 2 * bn ? step : 2.0 * bn);
+    const double epi = 1500 + (bn > 128 ? 2 : 1) * (act == SOUFFLE_ACT_GELU ? 1900 : 1000);
     const double cycles = waves * (loop > epi ? loop : epi) + epi;
-    if (cycles < least * 0.97) least = cycles, best = bn;
+    if (cycles < least) least = cycles, best = bn;
   }
   return best;
 }
@@ -495,19 +488,24 @@ static int pairs_launch(const LinearArgs& a, bool behind_quantisation, int sms, 
   if (tiles > (1 << 30)) return fail(SOUFFLE_BAD_SHAPE, "8-bit product of %d x %d: too many tiles", a.rows, a.cols);
   p.tiles = (int)tiles;
   int rc;
-  if ((rc = make_map(&p.x, a.x, a.rows, a.inner, a.x_stride, 128)) || (rc = make_map(&p.w, a.w, a.cols, a.inner, a.w_stride, p.bn / 2))) return rc;
+  constexpr CUtensorMapDataType bytes = CU_TENSOR_MAP_DATA_TYPE_UINT8, values = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+  if ((rc = make_map(&p.x, bytes, 1, a.x, a.rows, a.inner, a.x_stride, 128)) || (rc = make_map(&p.w, bytes, 1, a.w, a.cols, a.inner, a.w_stride, p.bn / 2))) return rc;
   const bool wide = ((uintptr_t)a.out & 15u) == 0 && (a.out_stride * (long long)sizeof(T)) % 16 == 0;
+  if (wide && (rc = make_map(&p.out, values, sizeof(T), a.out, a.rows, a.cols, a.out_stride * sizeof(T), 32))) return rc;
   auto fn = wide ? souffle_int8_pairs<T, true> : souffle_int8_pairs<T, false>;
   static bool ready[2][kMaxDevices];
   if (!ready[wide][dev]) {
-    SF_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+    SF_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairMostSmem));
     ready[wide][dev] = true;
   }
+  p.slot_bytes = kPairOperand + p.bn / 2 * 128;
+  const int room = (kPairMostSmem - kPairFixedSmem) / p.slot_bytes;
+  p.stages = room < kPairMaxStages ? room : kPairMaxStages;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(2 * (p.tiles < sms / 2 ? p.tiles : sms / 2));
   cfg.blockDim = dim3(kPairThreads);
-  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.dynamicSmemBytes = p.stages * p.slot_bytes + kPairFixedSmem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
