@@ -419,10 +419,11 @@ typedef struct SouffleInt8Linear {
   const float* w_scale;      /* [N] */
   const void* bias;          /* [N], or null */
   void* out;                 /* [M][N] */
-  void* workspace;           /* souffle_int8_linear_workspace_bytes(M, K, x_dtype), 16-byte aligned, no state between calls; null where that is 0 */
+  void* workspace;           /* souffle_int8_linear_workspace_bytes(M, K, N, x_dtype), 16-byte aligned, no state between calls; null where that is 0
+                                (quantised rows, and few floating ones, which need none) */
   size_t workspace_bytes;
 } SouffleInt8Linear;
-size_t souffle_int8_linear_workspace_bytes(int32_t rows, int32_t inner, int32_t x_dtype);
+size_t souffle_int8_linear_workspace_bytes(int32_t rows, int32_t inner, int32_t cols, int32_t x_dtype);
 int souffle_int8_linear_forward(const SouffleInt8Linear* call, souffle_stream_t stream);
 /* Blocks until `stream` is idle; SOUFFLE_DEVICE_TIMEOUT if, since the last such call on this device, a bounded wait of a product
  * has run out (its output is then undefined). */

@@ -134,7 +134,7 @@ SIGNATURES = {
     "souffle_residual_norm_status": (C.c_int, [C.c_void_p]),
     "souffle_int8_quantize_rows": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p,
                                              C.c_void_p]),
-    "souffle_int8_linear_workspace_bytes": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32]),
+    "souffle_int8_linear_workspace_bytes": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     "souffle_int8_linear_forward": (C.c_int, [C.c_void_p, C.c_void_p]),
     "souffle_int8_linear_status": (C.c_int, [C.c_void_p]),
 }

@@ -112,35 +112,46 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], int a0, int a1, int a2, int 
 }
 
 // A CTA has 16 channels and 8 kTok tokens; its warps take turns in the inner dimension, 64 columns at a time, and are added
-// through shared memory.  Weights and tokens come straight from memory in the operands' own layout, 16 bytes a lane: lane 4 g + t
-// holds columns 16 t .. 16 t + 15 of channels g and g + 8 and of token g, which both operands of the product agree on, so the order of
-// the columns inside the 64 does not matter to the sum.
-constexpr int kFewWarps = 8;
-template <int kTok>
-__global__ void __launch_bounds__(32 * kFewWarps) souffle_int8_few(const LinearArgs a) {
-  __shared__ int part[kFewWarps][kTok][16 * 8];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 8 * kTok;
-  const signed char* x = static_cast<const signed char*>(a.x);
-  int acc[kTok][4];
-#pragma unroll
-  for (int i = 0; i < kTok; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0;
+// through shared memory.  Weights come straight from memory in the operand's own layout, 16 bytes a lane: lane 4 g + t holds
+// columns 16 t .. 16 t + 15 of channels g and g + 8 and of token g, which both operands of the product agree on, so the order of
+// the columns inside the 64 does not matter to the sum.  What bounds it is the latency of memory: a warp asks for the weights of
+// kAhead chunks at once, the first ones before anything else.
+constexpr int kFewWarps = 8, kAhead = 4;
+struct FewSmem {
+  int part[kFewWarps][2][16 * 8];
+  float scale[16];
+  alignas(16) char box[kFewWarps][kTeamBox];
+};
+__device__ __forceinline__ void few_weights(const LinearArgs& a, int n0, int g, int t, int chunk, int4 (&w)[kAhead][2]) {
   const int4 none = make_int4(0, 0, 0, 0);
-  for (int k0 = 64 * warp; k0 < a.inner; k0 += 64 * kFewWarps) {
-    const int k = k0 + 16 * t;
-    const int4 w0 = n0 + g < a.cols ? load16(a.w + (n0 + g) * a.w_stride, k, a.inner) : none;
-    const int4 w1 = n0 + g + 8 < a.cols ? load16(a.w + (n0 + g + 8) * a.w_stride, k, a.inner) : none;
 #pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      const int m = m0 + 8 * i + g;
-      const int4 b = m < a.rows ? load16(x + m * a.x_stride, k, a.inner) : none;
-      mma_s8(acc[i], w0.x, w1.x, w0.y, w1.y, b.x, b.y);
-      mma_s8(acc[i], w0.z, w1.z, w0.w, w1.w, b.z, b.w);
-    }
+  for (int i = 0; i < kAhead; ++i) {
+    const int k = 64 * (chunk + i * kFewWarps) + 16 * t;
+    w[i][0] = k < a.inner && n0 + g < a.cols ? load16(a.w + (n0 + g) * a.w_stride, k, a.inner) : none;
+    w[i][1] = k < a.inner && n0 + g + 8 < a.cols ? load16(a.w + (n0 + g + 8) * a.w_stride, k, a.inner) : none;
   }
+}
+template <int kTok, class F> __device__ __forceinline__ void few_product(const LinearArgs& a, int n0, int warp, int g, int t, int4 (&w)[kAhead][2], int (&acc)[kTok][4], F token) {
+  const int chunks = (a.inner + 63) / 64;
+  for (int chunk = warp; chunk < chunks; chunk += kAhead * kFewWarps) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (chunk + i * kFewWarps >= chunks) break;
+#pragma unroll
+      for (int j = 0; j < kTok; ++j) {
+        const int4 b = token(j, 64 * (chunk + i * kFewWarps) + 16 * t);
+        mma_s8(acc[j], w[i][0].x, w[i][1].x, w[i][0].y, w[i][1].y, b.x, b.y);
+        mma_s8(acc[j], w[i][0].z, w[i][1].z, w[i][0].w, w[i][1].w, b.z, b.w);
+      }
+    }
+    if (chunk + kAhead * kFewWarps < chunks) few_weights(a, n0, g, t, chunk + kAhead * kFewWarps, w);
+  }
+}
+// The warps' sums become outputs; `scale` has the tokens' scales.
+template <int kTok> __device__ __forceinline__ void few_outputs(const LinearArgs& a, FewSmem& sm, int n0, int m0, int warp, int g, int t, const int (&acc)[kTok][4], const float* scale) {
 #pragma unroll
   for (int i = 0; i < kTok; ++i) {       // [token][channel]
-    int* p = part[warp][i];
+    int* p = sm.part[warp][i];
     p[(2 * t) * 16 + g] = acc[i][0];
     p[(2 * t + 1) * 16 + g] = acc[i][1];
     p[(2 * t) * 16 + g + 8] = acc[i][2];
@@ -148,15 +159,91 @@ __global__ void __launch_bounds__(32 * kFewWarps) souffle_int8_few(const LinearA
   }
   __syncthreads();
   for (int e = threadIdx.x; e < 128 * kTok; e += 32 * kFewWarps) {
-    const int m = m0 + (e >> 4), n = n0 + (e & 15);
+    const int token = e >> 4, m = m0 + token, n = n0 + (e & 15);
     if (m >= a.rows || n >= a.cols) continue;
     int sum = 0;
 #pragma unroll
-    for (int w = 0; w < kFewWarps; ++w) sum += part[w][e >> 7][e & 127];
-    float v = (float)sum * a.x_scale[m] * a.w_scale[n];
+    for (int w = 0; w < kFewWarps; ++w) sum += sm.part[w][e >> 7][e & 127];
+    float v = (float)sum * scale[token] * a.w_scale[n];
     if (a.bias) v += load_value(a.bias, a.out_dtype, n);
     store_value(a.out, a.out_dtype, m * a.out_stride + n, activate(v, a.act));
   }
+}
+
+// of rows that are quantised already
+template <int kTok>
+__global__ void __launch_bounds__(32 * kFewWarps) souffle_int8_few(const LinearArgs a) {
+  __shared__ FewSmem sm;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 8 * kTok;
+  const signed char* x = static_cast<const signed char*>(a.x);
+  int4 w[kAhead][2];
+  few_weights(a, n0, g, t, warp, w);
+  if (threadIdx.x < 8 * kTok) sm.scale[threadIdx.x] = m0 + (int)threadIdx.x < a.rows ? a.x_scale[m0 + threadIdx.x] : 0.0f;
+  int acc[kTok][4] = {};
+  few_product<kTok>(a, n0, warp, g, t, w, acc, [&](int j, int k) {
+    const int m = m0 + 8 * j + g;
+    return m < a.rows && k < a.inner ? load16(x + m * a.x_stride, k, a.inner) : make_int4(0, 0, 0, 0);
+  });
+  few_outputs<kTok>(a, sm, n0, m0, warp, g, t, acc, sm.scale);
+}
+
+// of floating rows, at most 8 kTok: each CTA quantises them for itself, into shared memory, a token by 8 / tokens warps (one launch, and no
+// rows or scales through memory).  kVec as in Columns.
+constexpr int kFewCached = 4, kFewFloatRows = 16, kFewFloatBytes = 96 * 1024;
+__host__ __device__ inline int few_pitch(int inner) {          // bytes of a token: zeros to a multiple of 64, an odd one, so that eight tokens' 64 bytes lie in all banks
+  const int n = (inner + 63) / 64;
+  return 64 * (n | 1);
+}
+template <class T, bool kVec, int kTok>
+__global__ void __launch_bounds__(32 * kFewWarps) souffle_int8_few_floats(const LinearArgs a, int warps_per_token) {
+  extern __shared__ __align__(16) signed char tokens[];
+  __shared__ FewSmem sm;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, n0 = blockIdx.x * 16;
+  int4 w[kAhead][2];
+  few_weights(a, n0, g, t, warp, w);
+  const int pitch = few_pitch(a.inner), teams = kFewWarps / warps_per_token, mine = warp / warps_per_token;
+  const Columns<kVec> cols = {(int)threadIdx.x - mine * 32 * warps_per_token, 32 * warps_per_token, a.inner};
+  Team team;
+  team.begin(sm.box[mine], warps_per_token, warp - mine * warps_per_token, 1 + mine, cols, 0);
+  for (int i = a.inner + threadIdx.x; i < pitch; i += 32 * kFewWarps)
+    for (int m = 0; m < a.rows; ++m) tokens[m * pitch + i] = 0;
+  if (warps_per_token > 1) team.meet();
+  const int groups = (a.inner + 256 * warps_per_token - 1) / (256 * warps_per_token);
+  for (int m = mine; m < a.rows; m += teams) {
+    const T* from = static_cast<const T*>(a.x) + m * a.x_stride;
+    signed char* to = tokens + m * pitch;
+    Eight<T> held[kFewCached];
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kFewCached; ++i) held[i] = cols.fetch(from, i);
+#pragma unroll
+    for (int i = 0; i < kFewCached; ++i) top = max_abs8(top, expand(held[i]));
+    for (int i = kFewCached; i < groups; ++i) top = max_abs8(top, cols.load(from, i));
+    const uint32_t most = team_max_bits(team, __float_as_uint(top) & 0x7fffffffu);
+    const RowScale rs = row_scale(most);
+    auto lay = [&](int i, const F8& x) {
+      const uint2 q = most < 0x7f800000u ? round_s8(x, rs.inv) : make_uint2(0u, 0u);
+      if (kVec) {
+        if (cols.has(i, 0)) *reinterpret_cast<uint2*>(to + cols.at(i, 0)) = q;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (cols.has(i, j)) to[cols.at(i, j)] = (signed char)((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < kFewCached; ++i) lay(i, expand(held[i]));
+    for (int i = kFewCached; i < groups; ++i) lay(i, cols.load(from, i));
+    if (cols.t == 0) sm.scale[m] = rs.scale;
+  }
+  __syncthreads();
+  int acc[kTok][4] = {};
+  few_product<kTok>(a, n0, warp, g, t, w, acc, [&](int j, int k) {
+    const int m = 8 * j + g;
+    return m < a.rows ? *reinterpret_cast<const int4*>(tokens + m * pitch + k) : make_int4(0, 0, 0, 0);
+  });
+  few_outputs<kTok>(a, sm, n0, 0, warp, g, t, acc, sm.scale);
 }
 
 // ---- many tokens -------------------------------------------------------------------------------------------------
@@ -516,8 +603,34 @@ static int pairs_launch(const LinearArgs& a, bool behind_quantisation, int sms, 
   return SOUFFLE_OK;
 }
 
-// Rows from which on the tensor cores' fifth generation is used
+// Up to kFewRows rows the legacy tensor path, which needs no tiles of 256 rows, is as fast or faster, as long as it does not read too many
+// weights (all of them for every sixteen rows): 64 x 768 x 3072 6.9 us against 7.3, but 48 x 4096 x 4096 20.2 against 10.7.
 constexpr int kFewRows = 64;
+constexpr long long kFewWeights = 12 << 20;
+static bool few_rows(int rows, int inner, int cols) {
+  return rows <= kFewRows && (rows <= 8 || (rows + 15) / 16 * (long long)inner * cols <= kFewWeights);
+}
+// Floating rows are quantised by every CTA for itself where that is less than a launch: values that CTAs read in all.  16 x 768 x 3072 5.2 us
+// (2.4 M), 16 x 4096 x 4096 12.9 (17 M).
+constexpr long long kFewFloatReads = 6 << 20;
+static bool few_floats(int rows, int inner, int cols) {
+  return rows <= kFewFloatRows && (long long)rows * few_pitch(inner) <= kFewFloatBytes && (long long)rows * inner * ((cols + 15) / 16) <= kFewFloatReads;
+}
+template <class T>
+static int few_launch(const LinearArgs& a, int dev, cudaStream_t st) {
+  const bool vec = a.inner % 8 == 0 && ((uintptr_t)a.x & 15u) == 0 && (a.x_stride * (long long)sizeof(T)) % 16 == 0;
+  const int warps = a.rows == 1 ? 8 : a.rows == 2 ? 4 : a.rows <= 4 ? 2 : 1, smem = a.rows * few_pitch(a.inner);
+  auto fn = a.rows <= 8 ? (vec ? souffle_int8_few_floats<T, true, 1> : souffle_int8_few_floats<T, false, 1>)
+                        : (vec ? souffle_int8_few_floats<T, true, 2> : souffle_int8_few_floats<T, false, 2>);
+  static bool ready[2][2][kMaxDevices];
+  if (!ready[a.rows <= 8][vec][dev]) {
+    SF_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewFloatBytes));
+    ready[a.rows <= 8][vec][dev] = true;
+  }
+  fn<<<(a.cols + 15) / 16, 32 * kFewWarps, smem, st>>>(a, warps);
+  SF_CUDA(cudaGetLastError());
+  return SOUFFLE_OK;
+}
 
 }  // namespace souffle
 
@@ -537,8 +650,8 @@ int souffle_int8_quantize_rows(const void* x, int32_t dtype, int64_t x_stride, i
   return quantise(x, dtype, x_stride, rows, cols, static_cast<signed char*>(q), q_stride, scale, (cudaStream_t)stream);
 }
 
-size_t souffle_int8_linear_workspace_bytes(int32_t rows, int32_t inner, int32_t x_dtype) {
-  if (rows < 1 || inner < 1 || x_dtype == SOUFFLE_I8) return 0;
+size_t souffle_int8_linear_workspace_bytes(int32_t rows, int32_t inner, int32_t cols, int32_t x_dtype) {
+  if (rows < 1 || inner < 1 || cols < 1 || x_dtype == SOUFFLE_I8 || few_floats(rows, inner, cols)) return 0;
   return (size_t)padded16(4LL * rows) + (size_t)rows * padded16(inner);       // scales, then quantised rows
 }
 
@@ -559,7 +672,7 @@ int souffle_int8_linear_forward(const SouffleInt8Linear* call, souffle_stream_t 
   if (!d.x || (given ? !aligned16(d.x) : (uintptr_t)d.x % value_size(d.x_dtype) != 0) || (uintptr_t)d.x_scale % 4 || !aligned16(d.w) || !d.w_scale ||
       (uintptr_t)d.w_scale % 4 || (uintptr_t)d.bias % oe || !d.out || (uintptr_t)d.out % oe)
     return fail(SOUFFLE_BAD_POINTER, "null or misaligned pointer");
-  const size_t need = souffle_int8_linear_workspace_bytes(d.rows, d.inner, d.x_dtype);
+  const size_t need = souffle_int8_linear_workspace_bytes(d.rows, d.inner, d.cols, d.x_dtype);
   if (need && (!aligned16(d.workspace) || d.workspace_bytes < need)) return fail(SOUFFLE_BAD_POINTER, "workspace is null, misaligned or smaller than souffle_int8_linear_workspace_bytes()");
   int sms, dev, rc = current_sms(&sms, &dev);
   if (rc) return rc;
@@ -568,13 +681,17 @@ int souffle_int8_linear_forward(const SouffleInt8Linear* call, souffle_stream_t 
   a.rows = d.rows; a.inner = d.inner; a.cols = d.cols; a.out_dtype = d.out_dtype; a.act = d.activation;
   a.x_stride = d.x_stride; a.w_stride = d.w_stride; a.out_stride = d.out_stride;
   a.x = d.x; a.x_scale = d.x_scale; a.w = static_cast<const signed char*>(d.w); a.w_scale = d.w_scale; a.bias = d.bias; a.out = d.out;
+  if (!given && few_floats(d.rows, d.inner, d.cols)) {
+    if (d.x_dtype == SOUFFLE_F32) return few_launch<float>(a, dev, st);
+    return d.x_dtype == SOUFFLE_F16 ? few_launch<__half>(a, dev, st) : few_launch<__nv_bfloat16>(a, dev, st);
+  }
   if (!given) {
     float* scale = static_cast<float*>(d.workspace);
     signed char* q = static_cast<signed char*>(d.workspace) + padded16(4LL * d.rows);
     if ((rc = quantise(d.x, d.x_dtype, d.x_stride, d.rows, d.inner, q, padded16(d.inner), scale, st))) return rc;
     a.x = q; a.x_scale = scale; a.x_stride = padded16(d.inner);
   }
-  if (d.rows > kFewRows) {
+  if (!few_rows(d.rows, d.inner, d.cols)) {
     if (d.out_dtype == SOUFFLE_F32) return pairs_launch<float>(a, !given, sms, dev, st);
     return d.out_dtype == SOUFFLE_F16 ? pairs_launch<__half>(a, !given, sms, dev, st) : pairs_launch<__nv_bfloat16>(a, !given, sms, dev, st);
   }

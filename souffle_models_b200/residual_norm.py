@@ -9,6 +9,7 @@ reference has the LayerNorm stages of its fused layer only (cpp/bert/kernels/fus
 """
 from __future__ import annotations
 
+import functools
 from typing import Dict, Optional, Tuple, Union
 
 import torch
@@ -16,79 +17,102 @@ import torch
 from . import _lib
 
 _NORMS = {"none": 0, "layer": 1, "rms": 2}
+_VECTORS = ("branch_weight", "branch_bias", "out_weight", "out_bias")
+_CODES, _rows_of, _pack, _pack_grad = _lib.DTYPE_CODES, _lib.rows_of, _lib.ResidualNorm.pack, _lib.ResidualNormGrad.pack
 
 
-def _vector(t: Optional[torch.Tensor], name: str, cols: int, dtype, device: int):
-    """(address, dtype) of an optional [cols] vector; `dtype`: what the vectors before it had."""
-    if t is None:
-        return 0, dtype
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(rows: int, cols: int, gate_rows: int) -> int:
+    return _lib.load().souffle_residual_norm_backward_workspace_bytes(rows, cols, gate_rows)
+
+
+def _vector(t: torch.Tensor, name: str, cols: int, device: int) -> int:
+    """Address of a [cols] vector."""
     if t.get_device() != device or not t.is_contiguous() or t.shape != (cols,):
         raise ValueError(f"{name} must be a contiguous CUDA tensor of {cols} values on the same device")
-    if dtype is not None and t.dtype != dtype:
-        raise ValueError(f"gate, weights and biases must share one type: {name} has {t.dtype}, others {dtype}")
-    return t.data_ptr(), t.dtype
+    return t.data_ptr()
 
 
-def _matrix(t: Optional[torch.Tensor], name: str, rows: int, cols: int, like: torch.Tensor):
-    """(address, stride) of an optional matrix of the branch's shape."""
-    if t is None:
-        return 0, 0
-    if t.dtype != like.dtype or t.get_device() != like.get_device():
+def _matrix(t: torch.Tensor, name: str, like: torch.Tensor, device: int):
+    """(address, stride) of a matrix of the branch's shape."""
+    if t.dtype != like.dtype or t.get_device() != device:
         raise ValueError(f"{name} must have the branch's type and device")
     if t.shape != like.shape:
         raise ValueError(f"{name} must have the branch's shape")
-    return t.data_ptr(), _lib.rows_of(t, name)[2]
+    return t.data_ptr(), _rows_of(t, name)[2]
 
 
 def _front(residual, branch, branch_norm, branch_weight, branch_bias, gate, out_norm, out_weight, out_bias, residual_scale, branch_scale,
            branch_eps, out_eps):
     """The checked head of a call record: (its first values without the outputs' strides, its input pointers, rows, columns, type of the
     vectors, gate rows)."""
-    code = _lib.DTYPE_CODES.get(branch.dtype)
-    if not branch.is_cuda or code is None:
+    dtype, dev = branch.dtype, branch.get_device()
+    code = _CODES.get(dtype)
+    if dev < 0 or code is None:
         raise ValueError("branch must be a float32, float16 or bfloat16 CUDA tensor")
-    if branch_norm not in _NORMS or out_norm not in _NORMS:
+    n1, n2 = _NORMS.get(branch_norm), _NORMS.get(out_norm)
+    if n1 is None or n2 is None:
         raise ValueError(f"norms are {', '.join(_NORMS)}: got {branch_norm}, {out_norm}")
-    rows, cols, ystride = _lib.rows_of(branch, "branch")
-    r, rstride = _matrix(residual, "residual", rows, cols, branch)
-    dev, dtype, g, gate_rows = branch.get_device(), None, 0, 0
+    rows, cols, ystride = _rows_of(branch, "branch")
+    r = rstride = g = gate_rows = w1 = b1 = w2 = b2 = 0
+    params = None
+    if residual is not None:
+        r, rstride = _matrix(residual, "residual", branch, dev)
     if gate is not None:
-        if gate.get_device() != dev or not gate.is_contiguous() or gate.dim() not in (1, 2) or gate.shape[-1] != cols:
+        shape = gate.shape
+        if gate.get_device() != dev or not gate.is_contiguous() or len(shape) not in (1, 2) or shape[-1] != cols:
             raise ValueError(f"gate must be a contiguous CUDA tensor [{cols}] or [gates, {cols}] on the branch's device")
-        g, dtype, gate_rows = gate.data_ptr(), gate.dtype, gate.shape[0] if gate.dim() == 2 else 1
+        g, params, gate_rows = gate.data_ptr(), gate.dtype, shape[0] if len(shape) == 2 else 1
         if not gate_rows or rows % gate_rows:
             raise ValueError(f"gate has {gate_rows} rows, which do not divide {rows}")
-    w1, dtype = _vector(branch_weight, "branch_weight", cols, dtype, dev)
-    b1, dtype = _vector(branch_bias, "branch_bias", cols, dtype, dev)
-    w2, dtype = _vector(out_weight, "out_weight", cols, dtype, dev)
-    b2, dtype = _vector(out_bias, "out_bias", cols, dtype, dev)
-    pcode = code if dtype is None else _lib.DTYPE_CODES.get(dtype, -1)
-    head = (rows, cols, code, pcode, _NORMS[branch_norm], _NORMS[out_norm], gate_rows, residual_scale, branch_scale, branch_eps, out_eps, 0,
-            rstride, ystride)
-    return head, (r, branch.data_ptr(), g, w1, b1, w2, b2), rows, cols, dtype, gate_rows
+    if branch_weight is not None:
+        w1 = _vector(branch_weight, "branch_weight", cols, dev)
+        params = _same(branch_weight, "branch_weight", params)
+    if branch_bias is not None:
+        b1 = _vector(branch_bias, "branch_bias", cols, dev)
+        params = _same(branch_bias, "branch_bias", params)
+    if out_weight is not None:
+        w2 = _vector(out_weight, "out_weight", cols, dev)
+        params = _same(out_weight, "out_weight", params)
+    if out_bias is not None:
+        b2 = _vector(out_bias, "out_bias", cols, dev)
+        params = _same(out_bias, "out_bias", params)
+    head = (rows, cols, code, code if params is None else _CODES.get(params, -1), n1, n2, gate_rows, residual_scale, branch_scale, branch_eps,
+            out_eps, 0, rstride, ystride)
+    return head, (r, branch.data_ptr(), g, w1, b1, w2, b2), rows, cols, params, gate_rows
+
+
+def _same(t: torch.Tensor, name: str, dtype):
+    """The one type of gate, weights and biases; `dtype`: what those before had."""
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"gate, weights and biases must share one type: {name} has {t.dtype}, others {dtype}")
+    return t.dtype
 
 
 def _forward(residual, branch, branch_norm, branch_weight, branch_bias, gate, out_norm, out_weight, out_bias, residual_scale, branch_scale,
              branch_eps, out_eps, keep_sum, quantize):
     head, ptrs, rows, cols, _, _ = _front(residual, branch, branch_norm, branch_weight, branch_bias, gate, out_norm, out_weight, out_bias,
                                           residual_scale, branch_scale, branch_eps, out_eps)
-    lib = _lib.load()
     stream = _lib.stream_on(branch.get_device())
-    shape = branch.shape
-    total = out = q = scale = None
+    shape, dtype, device = branch.shape, branch.dtype, branch.device
+    total = out = None
+    s_ptr = o_ptr = q_ptr = scale_ptr = q_stride = 0
     if keep_sum:
-        total = torch.empty(shape, dtype=branch.dtype, device=branch.device)
+        total = torch.empty(shape, dtype=dtype, device=device)
+        s_ptr = total.data_ptr()
     if quantize:
         from .int8 import empty_rows
-        q, scale = empty_rows(rows, cols, branch.device)
+        out = q, scale = empty_rows(rows, cols, device)
+        q_ptr, q_stride, scale_ptr = q.data_ptr(), (cols + 15) // 16 * 16, scale.data_ptr()
     elif out_norm != "none":
-        out = torch.empty(shape, dtype=branch.dtype, device=branch.device)
+        out = torch.empty(shape, dtype=dtype, device=device)
+        o_ptr = out.data_ptr()
     elif not keep_sum:
         raise ValueError("nothing to compute: neither the sum nor a norm of it is asked for")
-    _lib.check(lib.souffle_residual_norm_forward(_lib.ResidualNorm.pack(
-        *head, cols, cols, q.stride(0) if q is not None else 0, *ptrs, total.data_ptr() if keep_sum else 0, out.data_ptr() if out is not None else 0,
-        q.data_ptr() if q is not None else 0, scale.data_ptr() if q is not None else 0), stream))
-    return total, (q, scale) if quantize else out
+    rc = _lib.load().souffle_residual_norm_forward(_pack(*head, cols, cols, q_stride, *ptrs, s_ptr, o_ptr, q_ptr, scale_ptr), stream)
+    if rc:
+        _lib.check(rc)
+    return total, out
 
 
 class _Differentiable(torch.autograd.Function):
@@ -131,8 +155,11 @@ def residual_norm(residual: Optional[torch.Tensor], branch: torch.Tensor, *, bra
     serves rows / gates consecutive rows.  Weights, biases and gate are all of the branch's type or all float32.
     o is None without out_norm; with `quantize` it is (int8 rows, scales) for int8.int8_linear.  `keep_sum=False` leaves s out (None).
     Asynchronous.  Differentiable (not with quantize or without the sum) in all tensors."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (branch, residual, branch_weight, branch_bias, gate, out_weight,
-                                                                                  out_bias)):
+    if torch.is_grad_enabled() and (branch.requires_grad or (residual is not None and residual.requires_grad)
+                                    or (branch_weight is not None and branch_weight.requires_grad)
+                                    or (branch_bias is not None and branch_bias.requires_grad) or (gate is not None and gate.requires_grad)
+                                    or (out_weight is not None and out_weight.requires_grad)
+                                    or (out_bias is not None and out_bias.requires_grad)):
         if quantize or not keep_sum:
             raise ValueError("quantize and keep_sum=False have no gradient")
         return _Differentiable.apply(residual, branch, branch_weight, branch_bias, gate, out_weight, out_bias, branch_norm, out_norm,
@@ -151,27 +178,40 @@ def residual_norm_backward(grad_sum: Optional[torch.Tensor], grad_out: Optional[
     returned for every LayerNorm.  Entries for what is not there are None."""
     head, ptrs, rows, cols, dtype, gate_rows = _front(residual, branch, branch_norm, branch_weight, branch_bias, gate, out_norm, out_weight, None,
                                                       residual_scale, branch_scale, branch_eps, out_eps)
-    ds, ds_stride = _matrix(grad_sum, "grad_sum", rows, cols, branch)
-    do, do_stride = _matrix(grad_out, "grad_out", rows, cols, branch)
-    lib = _lib.load()
-    device = branch.device
-    stream = _lib.stream_on(branch.get_device())
-    dr = torch.empty(branch.shape, dtype=branch.dtype, device=device) if residual is not None else None
-    dy = torch.empty(branch.shape, dtype=branch.dtype, device=device)
-    # one allocation for the vectors' gradients: each begins on a multiple of 16 bytes where the vector path needs it
+    dev = branch.get_device()
+    ds = ds_stride = do = do_stride = dr_ptr = gate_ptr = 0
+    if grad_sum is not None:
+        ds, ds_stride = _matrix(grad_sum, "grad_sum", branch, dev)
+    if grad_out is not None:
+        do, do_stride = _matrix(grad_out, "grad_out", branch, dev)
+    stream = _lib.stream_on(dev)
+    device, shape, kind = branch.device, branch.shape, branch.dtype
+    d: Dict[str, Optional[torch.Tensor]] = dict.fromkeys(("branch_weight", "branch_bias", "gate", "out_weight", "out_bias", "residual"))
+    dy = torch.empty(shape, dtype=kind, device=device)
+    if residual is not None:
+        d["residual"] = dr = torch.empty(shape, dtype=kind, device=device)
+        dr_ptr = dr.data_ptr()
+    # one allocation for the vectors' gradients
     names = [n for n, there in (("branch_weight", branch_weight is not None), ("branch_bias", branch_norm == "layer"),
                                 ("out_weight", out_weight is not None), ("out_bias", out_norm == "layer")) if there]
-    d: Dict[str, Optional[torch.Tensor]] = dict.fromkeys(("branch_weight", "branch_bias", "gate", "out_weight", "out_bias"))
-    vectors = torch.empty(len(names), cols, dtype=dtype or branch.dtype, device=device)
-    d.update(zip(names, vectors.unbind(0)))
+    at = dict.fromkeys(_VECTORS, 0)
+    if names:
+        kind = dtype or kind
+        vectors = torch.empty((len(names), cols), dtype=kind, device=device)
+        base, step = vectors.data_ptr(), cols * kind.itemsize
+        for i, (n, t) in enumerate(zip(names, vectors.unbind(0))):
+            d[n], at[n] = t, base + i * step
     if gate is not None:
-        d["gate"] = torch.empty_like(gate)
-    ws = torch.empty(lib.souffle_residual_norm_backward_workspace_bytes(rows, cols, gate_rows), dtype=torch.uint8, device=device)
-    ptr = lambda t: 0 if t is None else t.data_ptr()
-    _lib.check(lib.souffle_residual_norm_backward(_lib.ResidualNormGrad.pack(
-        *head, 0, 0, 0, *ptrs, 0, 0, 0, 0, ds_stride, do_stride, cols, cols, ds, do, ptr(dr), dy.data_ptr(), ptr(d["gate"]), ptr(d["branch_weight"]),
-        ptr(d["branch_bias"]), ptr(d["out_weight"]), ptr(d["out_bias"]), ws.data_ptr(), ws.numel()), stream))
-    d["residual"], d["branch"] = dr, dy
+        d["gate"] = dg = torch.empty_like(gate)
+        gate_ptr = dg.data_ptr()
+    need = _workspace_bytes(rows, cols, gate_rows)
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    rc = _lib.load().souffle_residual_norm_backward(_pack_grad(
+        *head, 0, 0, 0, *ptrs, 0, 0, 0, 0, ds_stride, do_stride, cols, cols, ds, do, dr_ptr, dy.data_ptr(), gate_ptr, *at.values(), ws.data_ptr(), need),
+        stream)
+    if rc:
+        _lib.check(rc)
+    d["branch"] = dy
     return d
 
 

@@ -77,16 +77,17 @@ def test_workspaces_hold_what_the_kernels_write():
     assert lib.souffle_residual_norm_backward_workspace_bytes(0, 64, 0) == 0
     assert lib.souffle_residual_norm_backward_workspace_bytes(1, 64, 0) >= 5 * 64 * 4
     assert lib.souffle_residual_norm_backward_workspace_bytes(10 ** 6, 8192, 4) > lib.souffle_residual_norm_backward_workspace_bytes(10 ** 6, 8192, 1) > 0
-    assert lib.souffle_int8_linear_workspace_bytes(5, 100, _lib.I8) == 0
-    assert lib.souffle_int8_linear_workspace_bytes(5, 100, 1) >= 5 * 112 + 5 * 4
-    assert lib.souffle_int8_linear_workspace_bytes(1 << 20, 1 << 17, 1) > 1 << 37       # no 32-bit product on the way
+    assert lib.souffle_int8_linear_workspace_bytes(50, 100, 70, _lib.I8) == 0
+    assert lib.souffle_int8_linear_workspace_bytes(50, 100, 70, 1) >= 50 * 112 + 50 * 4
+    assert lib.souffle_int8_linear_workspace_bytes(5, 100, 70, 1) == 0                 # few floating rows are quantised where they are used
+    assert lib.souffle_int8_linear_workspace_bytes(1 << 20, 1 << 17, 1, 1) > 1 << 37       # no 32-bit product on the way
 
 
 @pytest.mark.parametrize("change,code", [
     (dict(rows=-1), 1), (dict(inner=0), 1), (dict(inner=131073, x_stride=131088, w_stride=131088), 1), (dict(cols=0), 1), (dict(x_dtype=4), 7), (dict(out_dtype=3), 7),
     (dict(activation=3), 7), (dict(x_stride=48), 1), (dict(x_stride=72), 1), (dict(w_stride=72), 1), (dict(out_stride=7), 1), (dict(x_scale=None), 7),
     (dict(x_dtype=1), 7), (dict(x=None), 2), (dict(x=4104), 2), (dict(w=4104), 2), (dict(w_scale=None), 2), (dict(bias=4097), 2), (dict(out=None), 2),
-    (dict(x_dtype=1, x_scale=None), 2), (dict(x_dtype=1, x_scale=None, workspace=4096, workspace_bytes=16), 2),
+    (dict(rows=40, x_dtype=1, x_scale=None), 2), (dict(rows=40, x_dtype=1, x_scale=None, workspace=4096, workspace_bytes=16), 2),
 ])
 def test_products_refuse(change, code):
     lib = _lib.load()
