@@ -5,8 +5,9 @@ There is no fallback: if the library is missing or a call fails, an exception is
 from __future__ import annotations
 
 import ctypes as C
+import importlib.machinery
+import importlib.util
 import os
-import struct
 
 import torch
 
@@ -53,30 +54,22 @@ class LstmDesc(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("layers", "hidden", "steps", "ref_input_delay", "timeout_ms")]
 
 
-class Record:
-    """A call record of the C ABI from one list of (name, kind), kind as in the struct module (i int32, f float, q int64, P pointer,
-    N size_t).  `pack(*values)` gives its bytes, which are passed as the record's address: packing 25 values takes 1.5 us where a
-    ctypes structure filled field by field takes 5, and the records of two threads never meet."""
-
-    _KINDS = {"i": C.c_int32, "f": C.c_float, "q": C.c_int64, "P": C.c_void_p, "N": C.c_size_t}
-
-    def __init__(self, fields):
-        self.structure = type("Structure", (C.Structure,), {"_fields_": [(n, self._KINDS[k]) for n, k in fields]})
-        self.pack = struct.Struct("@" + "".join(k for _, k in fields)).pack
+def _record(name: str, fields) -> type:
+    """A call record of the C ABI from (names, ctype) groups."""
+    return type(name, (C.Structure,), {"_fields_": [(n, t) for names, t in fields for n in names.split()]})
 
 
-_NORM_FIELDS = [(n, "i") for n in ("rows", "cols", "dtype", "param_dtype", "branch_norm", "out_norm", "gate_rows")] + \
-               [(n, "f") for n in ("residual_scale", "branch_scale", "branch_eps", "out_eps")] + [("reserved", "i")] + \
-               [(n, "q") for n in ("residual_stride", "branch_stride", "sum_stride", "out_stride", "out_q_stride")] + \
-               [(n, "P") for n in ("residual", "branch", "gate", "branch_weight", "branch_bias", "out_weight", "out_bias", "sum", "out",
-                                   "out_q", "out_scale")]
-ResidualNorm = Record(_NORM_FIELDS)
-ResidualNormGrad = Record(_NORM_FIELDS + [(n, "q") for n in ("grad_sum_stride", "grad_out_stride", "d_residual_stride", "d_branch_stride")] +
-                          [(n, "P") for n in ("grad_sum", "grad_out", "d_residual", "d_branch", "d_gate", "d_branch_weight", "d_branch_bias",
-                                              "d_out_weight", "d_out_bias", "workspace")] + [("workspace_bytes", "N")])
-Int8Linear = Record([(n, "i") for n in ("rows", "inner", "cols", "x_dtype", "out_dtype", "activation")] +
-                    [(n, "q") for n in ("x_stride", "w_stride", "out_stride")] +
-                    [(n, "P") for n in ("x", "x_scale", "w", "w_scale", "bias", "out", "workspace")] + [("workspace_bytes", "N")])
+_NORM_FIELDS = [("rows cols dtype param_dtype branch_norm out_norm gate_rows", C.c_int32),
+                ("residual_scale branch_scale branch_eps out_eps", C.c_float), ("reserved", C.c_int32),
+                ("residual_stride branch_stride sum_stride out_stride out_q_stride", C.c_int64),
+                ("residual branch gate branch_weight branch_bias out_weight out_bias sum out out_q out_scale", C.c_void_p)]
+ResidualNorm = _record("ResidualNorm", _NORM_FIELDS)
+ResidualNormGrad = _record("ResidualNormGrad", _NORM_FIELDS + [
+    ("grad_sum_stride grad_out_stride d_residual_stride d_branch_stride", C.c_int64),
+    ("grad_sum grad_out d_residual d_branch d_gate d_branch_weight d_branch_bias d_out_weight d_out_bias workspace", C.c_void_p),
+    ("workspace_bytes", C.c_size_t)])
+Int8Linear = _record("Int8Linear", [("rows inner cols x_dtype out_dtype activation", C.c_int32), ("x_stride w_stride out_stride", C.c_int64),
+                                    ("x x_scale w w_scale bias out workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)])
 
 DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 I8 = 3
@@ -164,6 +157,26 @@ def load() -> C.CDLL:
     return _lib
 
 
+_operators = None
+
+
+def operators():
+    """The module of the residual block's entry points (csrc/torch_binding.cpp), on the library that load() loads."""
+    global _operators
+    if _operators is None:
+        lib = load()
+        if _build.is_stale():
+            _build.build()
+        loader = importlib.machinery.ExtensionFileLoader("_operators", _build.BINDING_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_operators", loader))
+        loader.exec_module(module)
+        module.bind(*(C.cast(getattr(lib, "souffle_" + n), C.c_void_p).value for n in (
+            "int8_quantize_rows", "int8_linear_workspace_bytes", "int8_linear_forward", "residual_norm_forward",
+            "residual_norm_backward_workspace_bytes", "residual_norm_backward")))
+        _operators = module
+    return _operators
+
+
 # torch.cuda.current_stream() builds a Stream object, 3.2 us a call; the handle alone takes 0.3 us.  A blocking call on a small input
 # asks twice: squeeze-and-excite of 1 x 32 x 112 x 112, 8 us of kernel, took 32 us.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -174,35 +187,6 @@ def stream_ptr() -> int:
     if _raw_stream is None:
         return torch.cuda.current_stream().cuda_stream
     return _raw_stream(torch.cuda.current_device())
-
-
-_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
-
-
-def stream_on(device: int) -> int:
-    """Handle of the current stream of device number `device`, which has to be the current device: the library launches there."""
-    if device != _current_device():
-        raise ValueError(f"tensors are on device {device}, the current device is {torch.cuda.current_device()}")
-    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
-
-
-def rows_of(t: torch.Tensor, name: str, unit: int = 8):
-    """(rows, columns, elements from row to row) of a tensor whose last dimension is the columns: any contiguous one, or a
-    2-D one whose rows lie apart.  A lone row's stride means nothing; it is given as a multiple of `unit`."""
-    shape = t.shape
-    if len(shape) == 2:
-        rows, cols = shape
-        stride, step = t.stride()
-        if step != 1 and cols > 1:
-            raise ValueError(f"{name}: the last dimension must be contiguous")
-        if rows == 1:
-            stride = (cols + unit - 1) // unit * unit
-        return rows, cols, stride
-    if not shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous, or 2-D with contiguous rows")
-    cols = shape[-1]
-    rows = t.numel() // cols if cols else 0
-    return rows, cols, cols if rows != 1 else (cols + unit - 1) // unit * unit
 
 
 def check(code: int) -> None:

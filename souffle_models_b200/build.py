@@ -18,6 +18,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libsouffle_b200.so")
+BINDING_PATH = os.path.join(LIB_DIR, "_operators.so")      # the Python entry points of the residual block's operators, csrc/torch_binding.cpp
 
 NVCC_FLAGS = [
     "-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
@@ -40,10 +41,23 @@ def _sources():
 
 
 def is_stale() -> bool:
-    if not os.path.exists(LIB_PATH):
+    if not os.path.exists(LIB_PATH) or not os.path.exists(BINDING_PATH):
         return True
-    t = os.path.getmtime(LIB_PATH)
+    t = min(os.path.getmtime(LIB_PATH), os.path.getmtime(BINDING_PATH))
     return any(os.path.getmtime(s) > t for s in _sources())
+
+
+def _binding_command() -> list:
+    """g++ on torch_binding.cpp against the headers and libraries of the torch that is installed."""
+    import sysconfig
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")
+    return ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *(f"-I{d}" for d in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), cuda,
+                                 sysconfig.get_paths()["include"])),
+            "-o", BINDING_PATH, os.path.join(CSRC, "torch_binding.cpp"), f"-L{os.path.join(root, 'lib')}",
+            *(f"-l{n}" for n in ("c10", "c10_cuda", "torch_cpu", "torch_cuda", "torch_python"))]
 
 
 def _compile_all(out_dir: str, flags) -> str:
@@ -58,16 +72,20 @@ def _compile_all(out_dir: str, flags) -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compiles the translation units and links them into lib/libsouffle_b200.so."""
+    """Compiles the translation units and links them into lib/libsouffle_b200.so; beside it, lib/_operators.so."""
     if not force and not is_stale():
         return LIB_PATH
     os.makedirs(LIB_DIR, exist_ok=True)
+    binding = subprocess.Popen(_binding_command(), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     with tempfile.TemporaryDirectory() as tmp:
         said = _compile_all(tmp, [*NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else [])])
         res = subprocess.run([_nvcc(), *NVCC_FLAGS, "-shared", "-o", LIB_PATH, *(os.path.join(tmp, u[:-3] + ".o") for u in UNITS)],
                              capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
+    text = binding.communicate()[0]
+    if binding.returncode != 0:
+        raise RuntimeError("g++ failed:\n" + text)
     if verbose:
         sys.stderr.write(said)
     return LIB_PATH

@@ -1,0 +1,327 @@
+// The Python entry points of the residual block's operators over the C ABI: checks of the tensors, outputs and workspaces from torch's
+// allocator, the call on the current stream.  In C++ because these calls are short: on one token the same in Python around ctypes took
+// 10 us (a product) and 16 us (a norm) a call, most of them the host's.
+// The library's functions arrive as addresses (bind), so that this module and ctypes use the one library that was loaded.
+#define PY_SSIZE_T_CLEAN
+#include <Python.h>
+
+#include <ATen/core/Tensor.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/GradMode.h>
+#include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <stdarg.h>
+#include <stdio.h>
+#include <string.h>
+
+#include <stdexcept>
+#include <string>
+
+#include "../../include/souffle_b200.h"
+
+namespace {
+
+struct Library {
+  decltype(&souffle_int8_quantize_rows) quantize_rows;
+  decltype(&souffle_int8_linear_workspace_bytes) linear_workspace;
+  decltype(&souffle_int8_linear_forward) linear;
+  decltype(&souffle_residual_norm_forward) norm;
+  decltype(&souffle_residual_norm_backward_workspace_bytes) grad_workspace;
+  decltype(&souffle_residual_norm_backward) grad;
+} lib;
+
+struct BadValue : std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+struct BadType : std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+[[noreturn]] void refuse(const char* fmt, ...) {
+  char buf[400];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  throw BadValue(buf);
+}
+
+const at::Tensor* tensor_or_null(PyObject* o, const char* name) {
+  if (o == Py_None) return nullptr;
+  if (!THPVariable_Check(o)) throw BadType(std::string(name) + " must be a tensor");
+  return &THPVariable_Unpack(o);
+}
+const at::Tensor& tensor(PyObject* o, const char* name) {
+  const at::Tensor* t = tensor_or_null(o, name);
+  if (!t) throw BadType(std::string(name) + " must be a tensor");
+  return *t;
+}
+long long number(PyObject* o) {
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw std::bad_exception();
+  return v;
+}
+float real(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw std::bad_exception();
+  return (float)v;
+}
+
+int code_of(at::ScalarType t) {      // -1: none of the library's floating types
+  return t == at::kFloat ? SOUFFLE_F32 : t == at::kHalf ? SOUFFLE_F16 : t == at::kBFloat16 ? SOUFFLE_BF16 : -1;
+}
+at::ScalarType type_of(int code) { return code == SOUFFLE_F32 ? at::kFloat : code == SOUFFLE_F16 ? at::kHalf : at::kBFloat16; }
+
+// A tensor as rows: its last dimension are the columns; any contiguous one, or a 2-D one whose rows lie apart.
+struct Rows {
+  int64_t rows, cols, stride;        // a lone row's stride means nothing and is given as a multiple of `unit`
+};
+Rows rows_of(const at::Tensor& t, const char* name, int64_t unit) {
+  Rows r;
+  if (t.dim() == 2) {
+    r.rows = t.size(0), r.cols = t.size(1), r.stride = t.stride(0);
+    if (t.stride(1) != 1 && r.cols > 1) refuse("%s: the last dimension must be contiguous", name);
+  } else {
+    if (t.dim() == 0 || !t.is_contiguous()) refuse("%s must be contiguous, or 2-D with contiguous rows", name);
+    r.cols = t.size(-1), r.rows = r.cols ? t.numel() / r.cols : 0, r.stride = r.cols;
+  }
+  if (r.rows == 1) r.stride = (r.cols + unit - 1) / unit * unit;
+  if (r.rows > INT32_MAX || r.cols > INT32_MAX) refuse("%s has more than 2^31 rows or columns", name);
+  return r;
+}
+
+// The device that a call runs on: its tensors', which has to be the current one, for the library launches there.
+struct Where {
+  int device;
+  souffle_stream_t stream;
+  explicit Where(const at::Tensor& t) : device(t.get_device()) {
+    if (device != c10::cuda::current_device()) refuse("tensors are on device %d, the current device is %d", device, (int)c10::cuda::current_device());
+    stream = (souffle_stream_t)c10::cuda::getCurrentCUDAStream(device).stream();
+  }
+  at::Tensor empty(c10::IntArrayRef sizes, at::ScalarType type) const {
+    return at::Tensor(at::detail::empty_cuda(sizes, type, at::Device(at::kCUDA, device), std::nullopt));
+  }
+};
+void* address(const at::Tensor& t) { return t.defined() && t.numel() ? t.mutable_data_ptr() : nullptr; }
+const void* address(const at::Tensor* t) { return t ? t->const_data_ptr() : nullptr; }
+
+// a contiguous vector of n values on device `dev`
+void check_vector(const at::Tensor& t, const char* name, int64_t n, int dev) {
+  if (!t.is_cuda() || t.get_device() != dev || !t.is_contiguous() || t.dim() != 1 || t.size(0) != n)
+    refuse("%s must be a contiguous CUDA tensor of %lld values on the same device", name, (long long)n);
+}
+
+PyObject* wrap(const at::Tensor& t) {
+  if (!t.defined()) Py_RETURN_NONE;
+  return THPVariable_Wrap(t);
+}
+PyObject* tuple_of(std::initializer_list<at::Tensor> ts) {
+  PyObject* out = PyTuple_New((Py_ssize_t)ts.size());
+  Py_ssize_t i = 0;
+  for (const at::Tensor& t : ts) PyTuple_SET_ITEM(out, i++, wrap(t));
+  return out;
+}
+
+// Quantised rows begin on 16-byte boundaries: (the padded tensor, a view of its columns)
+at::Tensor quantised(const Where& at, int64_t rows, int64_t cols, at::Tensor* view) {
+  const int64_t pitch = (cols + 15) / 16 * 16;
+  at::Tensor room = at.empty({rows, pitch}, at::kChar);
+  *view = pitch == cols ? room : room.narrow(1, 0, cols);
+  return room;
+}
+
+PyObject* quantize_rows(PyObject* const* args) {
+  const at::Tensor& x = tensor(args[0], "x");
+  const int code = code_of(x.scalar_type());
+  if (!x.is_cuda() || code < 0) refuse("x must be a float32, float16 or bfloat16 CUDA tensor");
+  const Rows r = rows_of(x, "x", 8);
+  const Where at(x);
+  at::Tensor view, room = quantised(at, r.rows, r.cols, &view), scale = at.empty({r.rows}, at::kFloat);
+  const int rc = lib.quantize_rows(x.const_data_ptr(), code, r.stride, (int)r.rows, (int)r.cols, address(room), (r.cols + 15) / 16 * 16, (float*)address(scale), at.stream);
+  return rc ? PyLong_FromLong(rc) : tuple_of({view, scale});
+}
+
+// x, w, w_scale, bias, x_scale, activation, output's type (-1: x's, or fp16 for int8 rows)
+PyObject* int8_linear(PyObject* const* args) {
+  const at::Tensor &x = tensor(args[0], "x"), &w = tensor(args[1], "w"), &w_scale = tensor(args[2], "w_scale");
+  const at::Tensor *bias = tensor_or_null(args[3], "bias"), *x_scale = tensor_or_null(args[4], "x_scale");
+  SouffleInt8Linear d;
+  memset(&d, 0, sizeof(d));
+  const bool given = x.scalar_type() == at::kChar;
+  d.x_dtype = given ? (int)SOUFFLE_I8 : code_of(x.scalar_type());
+  if (!x.is_cuda() || d.x_dtype < 0) refuse("x must be an int8, float32, float16 or bfloat16 CUDA tensor");
+  d.activation = (int)number(args[5]);
+  d.out_dtype = (int)number(args[6]);
+  if (d.out_dtype < 0) d.out_dtype = given ? (int)SOUFFLE_F16 : d.x_dtype;
+  const at::ScalarType out_type = type_of(d.out_dtype);
+  const int dev = x.get_device();
+  const Rows rx = rows_of(x, "x", 16), rw = rows_of(w, "w", 16);
+  if (w.scalar_type() != at::kChar || w.dim() != 2 || rw.cols != rx.cols || !w.is_cuda() || w.get_device() != dev) refuse("w must be int8 [N, %lld] on x's device", (long long)rx.cols);
+  check_vector(w_scale, "w_scale", rw.rows, dev);
+  if (w_scale.scalar_type() != at::kFloat) refuse("w_scale must be float32");
+  if (given != (x_scale != nullptr)) refuse("x_scale comes with int8 rows and only with them");
+  if (given && (x_scale->scalar_type() != at::kFloat || x_scale->numel() != rx.rows || !x_scale->is_contiguous() || !x_scale->is_cuda() || x_scale->get_device() != dev))
+    refuse("x_scale must be a contiguous float32 tensor of %lld values on x's device", (long long)rx.rows);
+  if (bias) {
+    check_vector(*bias, "bias", rw.rows, dev);
+    if (bias->scalar_type() != out_type) refuse("bias must have the output's type");
+  }
+  const Where at(x);
+  c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = rw.rows;
+  at::Tensor out = at.empty(shape, out_type), ws;
+  d.rows = (int)rx.rows, d.inner = (int)rx.cols, d.cols = (int)rw.rows;
+  d.x_stride = rx.stride, d.w_stride = rw.stride, d.out_stride = rw.rows;
+  d.x = x.const_data_ptr(), d.x_scale = (const float*)address(x_scale), d.w = w.const_data_ptr(), d.w_scale = (const float*)w_scale.const_data_ptr();
+  d.bias = address(bias), d.out = address(out);
+  if (!given && (d.workspace_bytes = lib.linear_workspace(d.rows, d.inner, d.cols, d.x_dtype))) {
+    ws = at.empty({(int64_t)d.workspace_bytes}, at::kByte);
+    d.workspace = address(ws);
+  }
+  const int rc = lib.linear(&d, at.stream);
+  return rc ? PyLong_FromLong(rc) : wrap(out);
+}
+
+// The inputs of a norm call from args[0..6] residual, branch, branch_weight, branch_bias, gate, out_weight, out_bias; args[7..12] branch_norm,
+// out_norm, residual_scale, branch_scale, branch_eps, out_eps.
+struct NormCall {
+  SouffleResidualNorm d;
+  const at::Tensor *residual, *branch, *branch_weight, *branch_bias, *gate, *out_weight, *out_bias;
+  at::ScalarType params;             // of gate, weights and biases
+  bool differentiable = false;
+
+  const void* matrix(const at::Tensor* t, const char* name, int64_t* stride) const {
+    *stride = 0;
+    if (!t) return nullptr;
+    if (t->scalar_type() != branch->scalar_type() || !t->is_cuda() || t->get_device() != branch->get_device()) refuse("%s must have the branch's type and device", name);
+    if (t->sizes() != branch->sizes()) refuse("%s must have the branch's shape", name);
+    *stride = rows_of(*t, name, 8).stride;
+    return t->const_data_ptr();
+  }
+  const void* vector(const at::Tensor* t, const char* name, bool* first) {
+    if (!t) return nullptr;
+    check_vector(*t, name, d.cols, branch->get_device());
+    same(*t, name, first);
+    return t->const_data_ptr();
+  }
+  void same(const at::Tensor& t, const char* name, bool* first) {
+    if (!*first && t.scalar_type() != params) refuse("gate, weights and biases must share one type: %s has another one", name);
+    params = t.scalar_type();
+    *first = false;
+  }
+  explicit NormCall(PyObject* const* a) {
+    static const char* const names[7] = {"residual", "branch", "branch_weight", "branch_bias", "gate", "out_weight", "out_bias"};
+    const at::Tensor** const into[7] = {&residual, &branch, &branch_weight, &branch_bias, &gate, &out_weight, &out_bias};
+    const bool grads = c10::GradMode::is_enabled();
+    for (int i = 0; i < 7; ++i) {
+      *into[i] = i == 1 ? &tensor(a[i], names[i]) : tensor_or_null(a[i], names[i]);
+      differentiable = differentiable || (grads && *into[i] && (*into[i])->requires_grad());
+    }
+    memset(&d, 0, sizeof(d));
+    d.dtype = code_of(branch->scalar_type());
+    if (!branch->is_cuda() || d.dtype < 0) refuse("branch must be a float32, float16 or bfloat16 CUDA tensor");
+    const Rows r = rows_of(*branch, "branch", 8);
+    d.rows = (int)r.rows, d.cols = (int)r.cols, d.branch_stride = r.stride, d.branch = branch->const_data_ptr();
+    d.branch_norm = (int)number(a[7]), d.out_norm = (int)number(a[8]);
+    d.residual_scale = real(a[9]), d.branch_scale = real(a[10]), d.branch_eps = real(a[11]), d.out_eps = real(a[12]);
+    d.residual = matrix(residual, "residual", &d.residual_stride);
+    bool first = true;
+    params = branch->scalar_type();
+    if (gate) {
+      if (!gate->is_cuda() || gate->get_device() != branch->get_device() || !gate->is_contiguous() || gate->dim() < 1 || gate->dim() > 2 || gate->size(-1) != r.cols)
+        refuse("gate must be a contiguous CUDA tensor [%lld] or [gates, %lld] on the branch's device", (long long)r.cols, (long long)r.cols);
+      const int64_t gates = gate->dim() == 2 ? gate->size(0) : 1;
+      if (!gates || r.rows % gates) refuse("gate has %lld rows, which do not divide %lld", (long long)gates, (long long)r.rows);
+      d.gate = gate->const_data_ptr(), d.gate_rows = (int)gates;
+      same(*gate, "gate", &first);
+    }
+    d.branch_weight = vector(branch_weight, "branch_weight", &first);
+    d.branch_bias = vector(branch_bias, "branch_bias", &first);
+    d.out_weight = vector(out_weight, "out_weight", &first);
+    d.out_bias = vector(out_bias, "out_bias", &first);
+    d.param_dtype = code_of(params);
+  }
+};
+
+// the inputs, keep_sum, quantize -> (sum, out) or, quantised, (sum, rows, scales); NotImplemented where a gradient is wanted
+PyObject* residual_norm(PyObject* const* args) {
+  NormCall call(args);
+  const bool keep_sum = number(args[13]), quantise = number(args[14]);
+  if (call.differentiable) Py_RETURN_NOTIMPLEMENTED;
+  if (!keep_sum && !quantise && call.d.out_norm == SOUFFLE_NORM_NONE) refuse("nothing to compute: neither the sum nor a norm of it is asked for");
+  const Where at(*call.branch);
+  SouffleResidualNorm& d = call.d;
+  at::Tensor sum, out, view, scale;
+  d.sum_stride = d.out_stride = d.cols;
+  if (keep_sum) d.sum = address(sum = at.empty(call.branch->sizes(), call.branch->scalar_type()));
+  if (quantise) {
+    out = quantised(at, d.rows, d.cols, &view);
+    scale = at.empty({d.rows}, at::kFloat);
+    d.out_q = address(out), d.out_q_stride = (d.cols + 15) / 16 * 16, d.out_scale = (float*)address(scale);
+  } else if (d.out_norm != SOUFFLE_NORM_NONE) {
+    d.out = address(out = at.empty(call.branch->sizes(), call.branch->scalar_type()));
+  }
+  const int rc = lib.norm(&d, at.stream);
+  if (rc) return PyLong_FromLong(rc);
+  return quantise ? tuple_of({sum, view, scale}) : tuple_of({sum, out});
+}
+
+// the inputs (no out_bias), grad_sum, grad_out -> the gradients of residual, branch, branch_weight, branch_bias, gate, out_weight, out_bias
+PyObject* residual_norm_backward(PyObject* const* args) {
+  NormCall call(args);
+  SouffleResidualNormGrad g;
+  memset(&g, 0, sizeof(g));
+  g.f = call.d;
+  g.grad_sum = call.matrix(tensor_or_null(args[13], "grad_sum"), "grad_sum", &g.grad_sum_stride);
+  g.grad_out = call.matrix(tensor_or_null(args[14], "grad_out"), "grad_out", &g.grad_out_stride);
+  const Where at(*call.branch);
+  const at::ScalarType kind = call.branch->scalar_type();
+  at::Tensor dr, dy = at.empty(call.branch->sizes(), kind), dgate, vec[4];
+  g.d_branch = address(dy);
+  g.d_residual_stride = g.d_branch_stride = g.f.cols;
+  if (call.residual) g.d_residual = address(dr = at.empty(call.branch->sizes(), kind));
+  if (call.gate) g.d_gate = address(dgate = at.empty(call.gate->sizes(), call.params));
+  const bool there[4] = {call.branch_weight != nullptr, g.f.branch_norm == SOUFFLE_NORM_LAYER, call.out_weight != nullptr, g.f.out_norm == SOUFFLE_NORM_LAYER};
+  void** const to[4] = {&g.d_branch_weight, &g.d_branch_bias, &g.d_out_weight, &g.d_out_bias};
+  for (int i = 0; i < 4; ++i)
+    if (there[i]) *to[i] = address(vec[i] = at.empty({g.f.cols}, call.params));
+  g.workspace_bytes = lib.grad_workspace(g.f.rows, g.f.cols, g.f.gate_rows);
+  at::Tensor ws;
+  if (g.workspace_bytes) g.workspace = address(ws = at.empty({(int64_t)g.workspace_bytes}, at::kByte));
+  const int rc = lib.grad(&g, at.stream);
+  if (rc) return PyLong_FromLong(rc);
+  return tuple_of({dr, dy, vec[0], vec[1], dgate, vec[2], vec[3]});
+}
+
+PyObject* bind(PyObject* const* args) {
+  void** const to[6] = {(void**)&lib.quantize_rows, (void**)&lib.linear_workspace, (void**)&lib.linear, (void**)&lib.norm, (void**)&lib.grad_workspace, (void**)&lib.grad};
+  for (int i = 0; i < 6; ++i) *to[i] = (void*)(uintptr_t)number(args[i]);
+  Py_RETURN_NONE;
+}
+
+template <PyObject* (*kFunction)(PyObject* const*), int kArgs> PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != kArgs) return PyErr_Format(PyExc_TypeError, "%d arguments are wanted, got %zd", kArgs, n);
+  try {
+    return kFunction(args);
+  } catch (const BadValue& e) {
+    PyErr_SetString(PyExc_ValueError, e.what());
+  } catch (const BadType& e) {
+    PyErr_SetString(PyExc_TypeError, e.what());
+  } catch (const std::bad_exception&) {       // the interpreter has its own error set
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+  }
+  return nullptr;
+}
+
+template <PyObject* (*kFunction)(PyObject* const*), int kArgs> PyMethodDef method(const char* name) {
+  return {name, (PyCFunction)(void (*)(void))entry<kFunction, kArgs>, METH_FASTCALL, nullptr};
+}
+PyMethodDef methods[] = {method<bind, 6>("bind"), method<quantize_rows, 1>("quantize_rows"), method<int8_linear, 7>("int8_linear"),
+                         method<residual_norm, 15>("residual_norm"), method<residual_norm_backward, 15>("residual_norm_backward"), {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_operators", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__operators() { return PyModule_Create(&module); }

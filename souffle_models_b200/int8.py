@@ -8,7 +8,6 @@ layer or Swin block on them.
 """
 from __future__ import annotations
 
-import functools
 from typing import Optional, Tuple
 
 import torch
@@ -17,12 +16,6 @@ from . import _lib
 from .residual_norm import residual_norm
 
 _ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2}
-_CODES, _rows_of, _pack = _lib.DTYPE_CODES, _lib.rows_of, _lib.Int8Linear.pack
-
-
-@functools.lru_cache(maxsize=256)
-def _workspace_bytes(rows: int, inner: int, cols: int, code: int) -> int:
-    return _lib.load().souffle_int8_linear_workspace_bytes(rows, inner, cols, code)
 
 
 def empty_rows(rows: int, cols: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -35,14 +28,10 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """(q int8 [rows, cols], scale float32 [rows]) of x [..., cols] (float32, float16, bfloat16): with a = max |x| of a row,
     q = rint(x * min(127 / a, FLT_MAX)) and scale = a / 127; a row that holds an infinity or a NaN has scale NaN.  q's rows lie a
     multiple of 16 bytes apart.  Asynchronous."""
-    code = _lib.DTYPE_CODES.get(x.dtype)
-    if not x.is_cuda or code is None:
-        raise ValueError("x must be a float32, float16 or bfloat16 CUDA tensor")
-    rows, cols, stride = _lib.rows_of(x, "x")
-    lib, stream = _lib.load(), _lib.stream_on(x.get_device())
-    q, scale = empty_rows(rows, cols, x.device)
-    _lib.check(lib.souffle_int8_quantize_rows(x.data_ptr(), code, stride, rows, cols, q.data_ptr(), (cols + 15) // 16 * 16, scale.data_ptr(), stream))
-    return q, scale
+    got = _lib.operators().quantize_rows(x)
+    if got.__class__ is not tuple:
+        _lib.check(got)
+    return got
 
 
 def quantize_weight(w_kn: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -58,47 +47,13 @@ def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: O
     """x [..., K], int8 with `x_scale` [rows] (see quantize_rows) or floating (quantised on the way); w int8 [N, K] with rows a multiple
     of 16 bytes apart and w_scale [N] (see quantize_weight); bias [N] in the output's type; activation none, relu or gelu (tanh form).
     Returns [..., N] in `out_dtype`, by default x's type, float16 for int8 rows.  K <= 131072.  Asynchronous."""
-    dev, dtype = x.get_device(), x.dtype
-    given = dtype == torch.int8
-    code = _lib.I8 if given else _CODES.get(dtype)
-    if dev < 0 or code is None:
-        raise ValueError("x must be an int8, float32, float16 or bfloat16 CUDA tensor")
-    if out_dtype is None:
-        out_dtype = torch.float16 if given else dtype
-    out_code, act = _CODES.get(out_dtype), _ACTIVATIONS.get(activation)
-    if out_code is None or act is None:
+    act, out = _ACTIVATIONS.get(activation), -1 if out_dtype is None else _lib.DTYPE_CODES.get(out_dtype)
+    if act is None or out is None:
         raise ValueError(f"out_dtype is float32, float16 or bfloat16 and activation {', '.join(_ACTIVATIONS)}: got {out_dtype}, {activation}")
-    rows, inner, stride = _rows_of(x, "x", 16)
-    cols, w_inner, w_stride = _rows_of(w, "w", 16)
-    if w.dtype != torch.int8 or w_inner != inner or w.get_device() != dev:
-        raise ValueError(f"w must be int8 [N, {inner}] on x's device")
-    if w_scale.dtype != torch.float32 or w_scale.shape != (cols,) or not w_scale.is_contiguous() or w_scale.get_device() != dev:
-        raise ValueError(f"w_scale must be a contiguous float32 tensor of {cols} values on x's device")
-    x_scale_ptr = bias_ptr = ws_ptr = need = 0
-    if given != (x_scale is not None):
-        raise ValueError("x_scale comes with int8 rows and only with them")
-    if given:
-        if x_scale.dtype != torch.float32 or x_scale.numel() != rows or not x_scale.is_contiguous() or x_scale.get_device() != dev:
-            raise ValueError(f"x_scale must be a contiguous float32 tensor of {rows} values on x's device")
-        x_scale_ptr = x_scale.data_ptr()
-    if bias is not None:
-        if bias.dtype != out_dtype or bias.shape != (cols,) or not bias.is_contiguous() or bias.get_device() != dev:
-            raise ValueError(f"bias must be a contiguous {out_dtype} tensor of {cols} values on x's device")
-        bias_ptr = bias.data_ptr()
-    stream, device = _lib.stream_on(dev), x.device
-    shape = x.shape
-    out = torch.empty((rows, cols) if len(shape) == 2 else (*shape[:-1], cols), dtype=out_dtype, device=device)
-    if not given:
-        need = _workspace_bytes(rows, inner, cols, code)
-        if need:
-            ws = torch.empty(need, dtype=torch.uint8, device=device)
-            ws_ptr = ws.data_ptr()
-    rc = _lib.load().souffle_int8_linear_forward(_pack(
-        rows, inner, cols, code, out_code, act, stride, w_stride, cols, x.data_ptr(), x_scale_ptr, w.data_ptr(), w_scale.data_ptr(), bias_ptr,
-        out.data_ptr(), ws_ptr, need), stream)
-    if rc:
-        _lib.check(rc)
-    return out
+    got = _lib.operators().int8_linear(x, w, w_scale, bias, x_scale, act, out)
+    if got.__class__ is int:
+        _lib.check(got)
+    return got
 
 
 def status() -> None:

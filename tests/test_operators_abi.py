@@ -16,20 +16,20 @@ def test_call_records_have_the_headers_layout(tmp_path):
     src = '#include <stdio.h>\n#include <stddef.h>\n#include "souffle_b200.h"\nint main(void) {\n'
     for name, r in records.items():
         src += f'  printf("{name} %zu\\n", sizeof({name}));\n'
-        for f, _ in r.structure._fields_:
-            at = "f." + f if name == "SouffleResidualNormGrad" and f in dict(_lib.ResidualNorm.structure._fields_) else f
+        for f, _ in r._fields_:
+            at = "f." + f if name == "SouffleResidualNormGrad" and f in dict(_lib.ResidualNorm._fields_) else f
             src += f'  printf("{name}.{f} %zu\\n", offsetof({name}, {at}));\n'
     (tmp_path / "t.c").write_text(src + "  return 0;\n}\n")
     subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), "-o", str(tmp_path / "t"), str(tmp_path / "t.c")], check=True)
     out = dict(line.rsplit(" ", 1) for line in subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, check=True).stdout.splitlines())
     for name, r in records.items():
-        assert int(out[name]) == C.sizeof(r.structure) == len(r.pack(*([0] * len(r.structure._fields_))))
-        for f, _ in r.structure._fields_:
-            assert int(out[f"{name}.{f}"]) == getattr(r.structure, f).offset, f
+        assert int(out[name]) == C.sizeof(r)
+        for f, _ in r._fields_:
+            assert int(out[f"{name}.{f}"]) == getattr(r, f).offset, f
 
 
 def _norm(**kw):
-    d = _lib.ResidualNorm.structure(rows=4, cols=64, dtype=1, param_dtype=1, out_norm=1, residual_scale=1, branch_scale=1, branch_eps=1e-5, out_eps=1e-5,
+    d = _lib.ResidualNorm(rows=4, cols=64, dtype=1, param_dtype=1, out_norm=1, residual_scale=1, branch_scale=1, branch_eps=1e-5, out_eps=1e-5,
                                     residual_stride=64, branch_stride=64, sum_stride=64, out_stride=64, residual=4096, branch=8192, sum=12288, out=16384)
     for k, v in kw.items():
         setattr(d, k, v)
@@ -64,9 +64,9 @@ def test_null_records_and_empty_calls():
                                          (dict(out_norm=0, out=None), 2)])
 def test_gradients_refuse(change, code):
     lib = _lib.load()
-    d = _lib.ResidualNormGrad.structure()
+    d = _lib.ResidualNormGrad()
     front = _norm()
-    C.memmove(C.addressof(d), C.addressof(front), C.sizeof(_lib.ResidualNorm.structure))
+    C.memmove(C.addressof(d), C.addressof(front), C.sizeof(_lib.ResidualNorm))
     for k, v in change.items():
         setattr(d, k, v)
     assert lib.souffle_residual_norm_backward(C.addressof(d), None) == code, lib.souffle_last_error()
@@ -91,22 +91,11 @@ def test_workspaces_hold_what_the_kernels_write():
 ])
 def test_products_refuse(change, code):
     lib = _lib.load()
-    d = _lib.Int8Linear.structure(rows=4, inner=64, cols=8, x_dtype=_lib.I8, out_dtype=1, x_stride=64, w_stride=64, out_stride=8, x=4096, x_scale=4096, w=4096,
+    d = _lib.Int8Linear(rows=4, inner=64, cols=8, x_dtype=_lib.I8, out_dtype=1, x_stride=64, w_stride=64, out_stride=8, x=4096, x_scale=4096, w=4096,
                                   w_scale=4096, out=4096)
     for k, v in change.items():
         setattr(d, k, v)
     assert lib.souffle_int8_linear_forward(C.addressof(d), None) == code, lib.souffle_last_error()
-
-
-def test_rows_of_tensors():
-    rows_of = _lib.rows_of
-    x = torch.zeros(6, 20)
-    assert rows_of(x, "x") == (6, 20, 20) and rows_of(x[:, :7], "x") == (6, 7, 20) and rows_of(x.view(2, 3, 20), "x") == (6, 20, 20)
-    assert rows_of(x[:1, :7], "x") == (1, 7, 8) and rows_of(x[0, :7], "x", 16) == (1, 7, 16) and rows_of(x[::2], "x") == (3, 20, 40)
-    assert rows_of(x[:0], "x")[0] == 0
-    for bad in (x.t(), x.view(2, 3, 20)[:, :, :7], torch.zeros(())):
-        with pytest.raises(ValueError):
-            rows_of(bad, "x")
 
 
 def test_tensors_on_the_cpu_are_refused():
@@ -117,3 +106,7 @@ def test_tensors_on_the_cpu_are_refused():
         int8.quantize_rows(x)
     with pytest.raises(ValueError):
         int8.int8_linear(x, torch.zeros(8, 64, dtype=torch.int8), torch.zeros(8))
+    for bad in (lambda: int8.quantize_rows([1.0]), lambda: int8.int8_linear(None, x, x), lambda: residual_norm.residual_norm(x, None),
+                lambda: _lib.operators().int8_linear(x)):
+        with pytest.raises(TypeError):
+            bad()
