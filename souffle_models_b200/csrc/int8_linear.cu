@@ -24,7 +24,7 @@ struct LinearArgs {
 
 // A team of warps per row.  Rows of up to 8 kGroups columns a thread stay in registers between the search for the maximum and the
 // rounding; longer ones are read twice, the second time from L2.
-template <class T, bool kVec, int kGroups>
+template <class T, int kGroups>
 __global__ void __launch_bounds__(256) souffle_quantise_rows(const T* __restrict__ x, long long x_stride, int rows, int cols_n, signed char* q,
                                                              long long q_stride, float* scale, int warps_per_row) {
   __shared__ __align__(16) char box[kTeamBox];
@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(256) souffle_quantise_rows(const T* __restrict
   if (row >= rows) return;
   const T* from = x + row * x_stride;
   signed char* to = q + row * q_stride;
-  const Columns<kVec> cols = {(int)(threadIdx.x % (32 * warps_per_row)), 32 * warps_per_row, cols_n};
+  const Columns<true> cols = {(int)(threadIdx.x % (32 * warps_per_row)), 32 * warps_per_row, cols_n};
   Team team;
   team.begin(box, warps_per_row, warp % warps_per_row, 1, cols, 0);
   if (warps_per_row > 1) team.meet();
@@ -53,15 +53,60 @@ __global__ void __launch_bounds__(256) souffle_quantise_rows(const T* __restrict
   const bool fine = most < 0x7f800000u;
   for (int i = 0; i < groups; ++i) {
     const uint2 w = fine ? round_s8(cols.load(from, i), rs.inv) : make_uint2(0u, 0u);
-    if (kVec) {
-      if (cols.has(i, 0)) *reinterpret_cast<uint2*>(to + cols.at(i, 0)) = w;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (cols.has(i, j)) to[cols.at(i, j)] = (signed char)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
-    }
+    if (cols.has(i, 0)) *reinterpret_cast<uint2*>(to + cols.at(i, 0)) = w;
   }
   if (threadIdx.x % (32 * warps_per_row) == 0) scale[row] = rs.scale;
+}
+
+// The same for rows that begin anywhere: a team reads neighbouring values one a lane, the first 16 a lane stay in registers, and the
+// bytes, which begin on a boundary, go out through shared memory 16 at a time.  (Bytes stored one by one: 3000 x 3333 fp32 40 us.)
+constexpr int kOddHeld = 16, kOddBytes = 4096;       // of a row that pass shared memory; what is behind them is stored byte by byte
+template <class T>
+__global__ void __launch_bounds__(256) souffle_quantise_rows_any(const T* __restrict__ x, long long x_stride, int rows, int cols, signed char* q,
+                                                                 long long q_stride, float* scale, int warps_per_row) {
+  __shared__ __align__(16) signed char bytes[8][kOddBytes / 8];
+  __shared__ uint32_t most_of[8];
+  const int team = 32 * warps_per_row, mine = threadIdx.x / team, t = threadIdx.x - mine * team;
+  const int row = blockIdx.x * (256 / team) + mine;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (row >= rows) return;
+  auto meet = [&] {
+    if (warps_per_row == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + mine), "r"(team) : "memory");
+  };
+  const T* from = x + row * x_stride;
+  signed char *to = q + row * q_stride, *own = &bytes[mine * warps_per_row][0];
+  float v[kOddHeld], top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kOddHeld; ++i) v[i] = t + i * team < cols ? to_f32(from[t + i * team]) : 0.0f;
+#pragma unroll
+  for (int i = 0; i < kOddHeld; ++i) top = max_abs(top, v[i]);
+#pragma unroll 4
+  for (int c = t + kOddHeld * team; c < cols; c += team) top = max_abs(top, to_f32(from[c]));
+  uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top) & 0x7fffffffu);
+  if (warps_per_row > 1) {
+    if ((threadIdx.x & 31) == 0) most_of[threadIdx.x >> 5] = most;
+    meet();
+    for (int w = 0; w < warps_per_row; ++w) most = max(most, most_of[mine * warps_per_row + w]);
+  }
+  const RowScale rs = row_scale(most);
+  const bool fine = most < 0x7f800000u;
+  auto round = [&](float f) { return (signed char)(fine ? __float_as_uint(__fadd_rn(__fmul_rn(f, rs.inv), 12582912.0f)) : 0u); };
+#pragma unroll
+  for (int i = 0; i < kOddHeld; ++i)
+    if (t + i * team < cols) own[t + i * team] = round(v[i]);
+#pragma unroll 4
+  for (int c = t + kOddHeld * team; c < cols; c += team) to[c] = round(to_f32(from[c]));
+  meet();
+  const int held = cols < kOddHeld * team ? cols : kOddHeld * team;
+  for (int c = 16 * t; c < held; c += 16 * team) {
+    if (c + 16 <= held) {
+      *reinterpret_cast<uint4*>(to + c) = *reinterpret_cast<const uint4*>(own + c);
+    } else {
+      for (int i = c; i < held; ++i) to[i] = own[i];
+    }
+  }
+  if (t == 0) scale[row] = rs.scale;
 }
 
 // ---- epilogue ----------------------------------------------------------------------------------------------------
@@ -479,13 +524,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) sou
             }
           } else {                     // rows begin anywhere: the lanes write neighbouring elements
             __syncwarp();
-            const int held = ends + n0 - n < kBoxCols ? ends + n0 - n : kBoxCols;
-            for (int c = lane; c < held; c += 32)
+            const int held = ends + n0 - n < kBoxCols ? ends + n0 - n : kBoxCols, rows = a.rows - m0 < 32 ? a.rows - m0 : 32;
+            for (int c = lane; c < held; c += 32) {
+              const int byte = c * (int)sizeof(T);
+              T* out = static_cast<T*>(a.out) + m0 * a.out_stride + n + c;
+#pragma unroll 8
               for (int row = 0; row < 32; ++row) {
-                if (m0 + row >= a.rows) break;
-                const int byte = c * (int)sizeof(T);
-                static_cast<T*>(a.out)[(m0 + row) * a.out_stride + n + c] = *reinterpret_cast<const T*>(at + row * 128 + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15));
+                const T value = *reinterpret_cast<const T*>(at + row * 128 + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15));
+                if (row < rows) out[row * a.out_stride] = value;
               }
+            }
             __syncwarp();
           }
         }
@@ -518,14 +566,19 @@ constexpr int kMaxInner = 131072;
 template <class T>
 static int quantise_launch(const T* x, long long x_stride, int rows, int cols, signed char* q, long long q_stride, float* scale, cudaStream_t st) {
   const bool vec = cols % 8 == 0 && ((uintptr_t)x & 15u) == 0 && (x_stride * (long long)sizeof(T)) % 16 == 0;
-  const int groups8 = (cols + 7) / 8;
+  if (!vec) {
+    const int need = (cols + 32 * kOddHeld - 1) / (32 * kOddHeld), warps = need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : 8, teams = 8 / warps;
+    souffle_quantise_rows_any<T><<<(rows + teams - 1) / teams, 256, 0, st>>>(x, x_stride, rows, cols, q, q_stride, scale, warps);
+    SF_CUDA(cudaGetLastError());
+    return SOUFFLE_OK;
+  }
+  const int groups8 = cols / 8;
   int warps = (groups8 + 127) / 128;
   if (warps > 8) warps = 8;
   const int threads = warps == 1 ? 128 : 32 * warps, teams = threads / (32 * warps), grid = (rows + teams - 1) / teams;
   const int groups = (groups8 + 32 * warps - 1) / (32 * warps);
   auto go = [&](auto fn) { fn<<<grid, threads, 0, st>>>(x, x_stride, rows, cols, q, q_stride, scale, warps); };
-  if (vec) groups <= 1 ? go(souffle_quantise_rows<T, true, 1>) : groups == 2 ? go(souffle_quantise_rows<T, true, 2>) : groups == 3 ? go(souffle_quantise_rows<T, true, 3>) : go(souffle_quantise_rows<T, true, 4>);
-  else groups <= 1 ? go(souffle_quantise_rows<T, false, 1>) : groups == 2 ? go(souffle_quantise_rows<T, false, 2>) : go(souffle_quantise_rows<T, false, 4>);
+  groups <= 1 ? go(souffle_quantise_rows<T, 1>) : groups == 2 ? go(souffle_quantise_rows<T, 2>) : groups == 3 ? go(souffle_quantise_rows<T, 3>) : go(souffle_quantise_rows<T, 4>);
   SF_CUDA(cudaGetLastError());
   return SOUFFLE_OK;
 }

@@ -119,17 +119,6 @@ template <class T> __device__ __forceinline__ Eight<T> narrow(const F8& a) {
   for (int i = 0; i < 4; ++i) put_pair(e, i, halves(a.p[i]));
   return e;
 }
-// one of the eight
-template <class T> __device__ __forceinline__ T value_of(const Eight<T>& e, int j) {
-  T v;
-  if (sizeof(T) == 4) {
-    memcpy(&v, &e.w[j], 4);
-  } else {
-    const uint16_t bits = (uint16_t)(e.w[j >> 1] >> (16 * (j & 1)));
-    memcpy(&v, &bits, 2);
-  }
-  return v;
-}
 template <class T> __device__ __forceinline__ void put_value(Eight<T>& e, int j, const T* p) {      // into zeros
   if (sizeof(T) == 4) e.w[j] = *reinterpret_cast<const uint32_t*>(p);
   else e.w[j >> 1] |= (uint32_t)*reinterpret_cast<const uint16_t*>(p) << (16 * (j & 1));
@@ -174,15 +163,22 @@ template <bool kVec_> struct Columns {
     }
     return e;
   }
-  template <class T> __device__ __forceinline__ F8 load(const T* row, int i) const { return expand(fetch(row, i)); }
-  template <class T> __device__ __forceinline__ void store(T* row, int i, const F8& v) const {
-    const Eight<T> e = narrow<T>(v);
+  template <class T> __device__ __forceinline__ F8 load(const T* row, int i) const {
+    if (kVec) return expand(fetch(row, i));
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = has(i, j) ? to_f32(row[at(i, j)]) : 0.0f;
+    return pack8(v);
+  }
+  template <class T> __device__ __forceinline__ void store(T* row, int i, const F8& x) const {
     if (kVec) {
-      if (has(i, 0)) write16(row + at(i, 0), e);
+      if (has(i, 0)) write16(row + at(i, 0), narrow<T>(x));
     } else {
+      float v[8];
+      unpack8(x, v);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (has(i, j)) row[at(i, j)] = value_of(e, j);
+        if (has(i, j)) row[at(i, j)] = from_f32<T>(v[j]);
     }
   }
   // 1, or 0 where the thread has none of group i: with kVec it has all eight columns or none, and a factor keeps what lies past the
