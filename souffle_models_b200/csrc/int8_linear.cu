@@ -299,7 +299,6 @@ __global__ void __launch_bounds__(32 * kFewWarps) souffle_int8_few_floats(const 
 // tile's are computed in the other half of tensor memory, 32 rows x 32 columns at a time and each by itself.  Zeros past the
 // matrices' ends come from the copy engine.
 constexpr int kPairMaxStages = 8, kPairOperand = 128 * 128, kPairBox = 4096, kParts = 2 /* epilogue warps a lane quarter */, kPairThreads = 64 + 128 * kParts;
-constexpr unsigned long long kPairTimeoutNs = 2000000000ull;
 struct PairCtl {
   uint64_t full[kPairMaxStages], empty[kPairMaxStages], tmem_full[2], tmem_empty[2];
   WaitCtl wait;
@@ -315,6 +314,7 @@ struct PairArgs {
   LinearArgs a;
   int bn, tiles_n, tiles, chunks;
   int stages, slot_bytes;              // of the ring
+  unsigned long long timeout_ns;       // after which waits give up, from a CTA's start on
 };
 // Where a tile lies, in tiles; the next one of a pair is step_m rows and step_n columns of tiles further (divisions take a warp 150
 // cycles each).
@@ -360,7 +360,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) sou
     cs.abort = 0;
     cs.wait.abort_smem = &cs.abort;
     cs.wait.status_g = g_linear_status;
-    cs.wait.deadline_ns = globaltimer_ns() + kPairTimeoutNs;
+    cs.wait.deadline_ns = globaltimer_ns() + p.timeout_ns;
     fence_mbar_init();
   }
   if (warp == 1) tmem_alloc_pair(smem_u32(&cs.tmem_base), 512);
@@ -561,7 +561,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) sou
 
 static bool is_float_type(int t) { return t >= SOUFFLE_F32 && t <= SOUFFLE_BF16; }
 static size_t value_size(int t) { return t == SOUFFLE_F32 ? 4 : 2; }
-constexpr int kMaxInner = 131072;
+constexpr int kMaxInner = 131072, kMaxRows = 1 << 30;
 
 template <class T>
 static int quantise_launch(const T* x, long long x_stride, int rows, int cols, signed char* q, long long q_stride, float* scale, cudaStream_t st) {
@@ -627,6 +627,8 @@ static int pairs_launch(const LinearArgs& a, bool behind_quantisation, int sms, 
   const long long tiles = (long long)((a.rows + 255) / 256) * p.tiles_n;
   if (tiles > (1 << 30)) return fail(SOUFFLE_BAD_SHAPE, "8-bit product of %d x %d: too many tiles", a.rows, a.cols);
   p.tiles = (int)tiles;
+  // two seconds beside the work itself at a thirtieth of the measured rate
+  p.timeout_ns = 2000000000ull + (unsigned long long)(2e-5 * a.rows * (double)a.inner * a.cols);
   int rc;
   constexpr CUtensorMapDataType bytes = CU_TENSOR_MAP_DATA_TYPE_UINT8, values = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
   if ((rc = make_map(&p.x, bytes, 1, a.x, a.rows, a.inner, a.x_stride, 128)) || (rc = make_map(&p.w, bytes, 1, a.w, a.cols, a.inner, a.w_stride, p.bn / 2))) return rc;
@@ -711,8 +713,8 @@ size_t souffle_int8_linear_workspace_bytes(int32_t rows, int32_t inner, int32_t 
 int souffle_int8_linear_forward(const SouffleInt8Linear* call, souffle_stream_t stream) {
   if (!call) return fail(SOUFFLE_BAD_ARGUMENT, "null call record");
   const SouffleInt8Linear& d = *call;
-  if (d.rows < 0 || d.cols < 1 || d.inner < 1 || d.inner > kMaxInner)
-    return fail(SOUFFLE_BAD_SHAPE, "8-bit product of %d x %d x %d: rows >= 0, cols >= 1 and 1 <= inner <= %d are wanted", d.rows, d.cols, d.inner, kMaxInner);
+  if (d.rows < 0 || d.rows > kMaxRows || d.cols < 1 || d.cols > kMaxRows || d.inner < 1 || d.inner > kMaxInner)
+    return fail(SOUFFLE_BAD_SHAPE, "8-bit product of %d x %d x %d: 0 <= rows and 1 <= cols, at most %d, and 1 <= inner <= %d are wanted", d.rows, d.inner, d.cols, kMaxRows, kMaxInner);
   if (!(is_float_type(d.x_dtype) || d.x_dtype == SOUFFLE_I8) || !is_float_type(d.out_dtype))
     return fail(SOUFFLE_BAD_ARGUMENT, "x_dtype %d, out_dtype %d: rows are int8, fp32, fp16 or bf16, outputs fp32, fp16 or bf16", d.x_dtype, d.out_dtype);
   if (d.activation < SOUFFLE_ACT_NONE || d.activation > SOUFFLE_ACT_GELU) return fail(SOUFFLE_BAD_ARGUMENT, "activation %d is none of SOUFFLE_ACT_*", d.activation);

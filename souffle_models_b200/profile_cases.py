@@ -18,13 +18,14 @@ bert_layer_s384
 (the reference's native shape and numerical variant through the blocking drop-in entry, which also returns the five
 intermediate tensors), bert_layer_s384_plan (the same launch called back to back), lstm (10 x 256, 100 steps), swin_mlp (256 x 512 x 2048),
 swin_pair (14 x 14 x 512, shifts 0 and 3), swin_stage (18 blocks + patch merging), se_module (the reference's ten
-shapes, one call each per round).
+shapes, one call each per round), int8_mlp (the MLP half of a BERT layer on 8-bit products, 8192 tokens of 768: quantisation, two products,
+norm), int8_mlp_b1 (one token), residual_norm and residual_norm_grad (8192 x 768, fp16).
 """
 import sys
 
 import torch
 
-from . import bert, efficientnet, lstm, swin
+from . import bert, efficientnet, int8, lstm, residual_norm, swin
 
 SE_SHAPES = [(112, 32, 8), (56, 96, 4), (56, 144, 6), (28, 144, 6), (28, 240, 10), (14, 240, 10), (14, 480, 20),
              (14, 672, 28), (7, 672, 28), (7, 1152, 48)]      # (height = width, channels, reduce channels)
@@ -110,6 +111,18 @@ def make_case(name: str):
         plan = swin.SwinBlock(1, 14, 512, 16, 7, 0, blocks, shift_alt=3, merge=merge)
         x = _h((196, 512), g)
         return (lambda: plan.forward(x)), plan.status
+    if name in ("int8_mlp", "int8_mlp_b1"):
+        w = _bert_layers(1, 768, 3072, g, True)[0]
+        mlp = int8.Int8Mlp(w["fc1_w"], w["fc1_b"], w["fc2_w"], w["fc2_b"], w["ln2_g"], w["ln2_b"], eps=1e-12)
+        x = _h((8192 if name == "int8_mlp" else 1, 768), g)
+        return (lambda: mlp.forward(x)), int8.status
+    if name in ("residual_norm", "residual_norm_grad"):
+        r, y, ds, do = (_h((8192, 768), g) for _ in range(4))
+        w, b = 1 + _h((768,), g, 0.1), _h((768,), g, 0.1)
+        kw = dict(out_norm="layer", out_weight=w)
+        if name == "residual_norm":
+            return (lambda: residual_norm.residual_norm(r, y, out_bias=b, **kw)), residual_norm.status
+        return (lambda: residual_norm.residual_norm_backward(ds, do, r, y, **kw)), residual_norm.status
     if name == "se_module":
         cases = [(torch.randn(1, c, hw, hw, generator=g).cuda(), (torch.randn(r, c, generator=g) * 0.1).cuda(),
                   (torch.randn(c, r, generator=g) * 0.1).cuda()) for hw, c, r in SE_SHAPES]
