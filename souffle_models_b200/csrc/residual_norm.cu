@@ -114,6 +114,8 @@ __global__ void __launch_bounds__(1024) souffle_residual_norm_any(const NormArgs
 
 constexpr unsigned long long kRowTimeoutNs = 2000000000ull;
 constexpr int kMaxRowSlots = 4;
+// Two rows at a time hold two slots: fewer than this leave none for the rows behind them.
+constexpr int kTwoSlots = 4;
 // {code, where, cta, 0} of the first wait that ran out since the status was last read
 __device__ int g_norm_status[4];
 
@@ -146,6 +148,7 @@ struct RowPlan {
   int warps, teams, total_teams, slots;        // of a row; of a CTA; of the grid; of a team's ring
   int row_bytes, operands;                     // of one operand's row; operands of a row in the ring
   int team_bytes, vectors;                     // shared memory of a team; where the vectors begin
+  int rows_each, rows_over;                    // rows / total_teams and rows % total_teams
 };
 // shared memory: RowCtl (64 bytes), then each team's box, barriers, gate and ring, then the vectors
 __host__ __device__ inline int team_gate_at() { return kTeamBox + kMaxRowSlots * 8; }
@@ -215,8 +218,11 @@ template <int kVectors> __device__ __forceinline__ void lay_vectors(float* to, c
   }
 }
 
-template <class T, bool kFull, int kGroups, bool kN1>
-__global__ void __launch_bounds__(768, 1) souffle_residual_norm_rows(const NormArgs a, const RowPlan p) {
+// kTwo: rows that one warp holds, two at a time on sixteen warps; wider ones one by one on twenty-four (8192 x 768 fp16 15.0 -> 13.9 us,
+// 8192 x 264 with both norms 12.5 -> 10.2, but 4095 x 4096 bf16 28.1 -> 31.5).
+constexpr int row_warps(bool two) { return two ? 16 : 24; }
+template <class T, bool kFull, int kGroups, bool kN1, bool kTwo>
+__global__ void __launch_bounds__(32 * row_warps(kTwo), 1) souffle_residual_norm_rows(const NormArgs a, const RowPlan p) {
   extern __shared__ __align__(128) char smem[];
   RowCtl& ctl = *reinterpret_cast<RowCtl*>(smem);
   const int warp = threadIdx.x >> 5, mine = warp / p.warps, t = threadIdx.x - mine * 32 * p.warps;
@@ -228,15 +234,19 @@ __global__ void __launch_bounds__(768, 1) souffle_residual_norm_rows(const NormA
   const float *vec = reinterpret_cast<const float*>(smem + p.vectors), *vec_s = vec + plane_at(cols.first);
   const bool have_r = a.r != nullptr, have_gate = a.gate != nullptr;
   RowRing<2> ring;
-  ring.step[0] = p.total_teams * a.y_stride * (long long)sizeof(T);
-  ring.step[1] = p.total_teams * a.r_stride * (long long)sizeof(T);
-  ring.from[0] = static_cast<const char*>(a.y) + id * a.y_stride * (long long)sizeof(T);
-  ring.from[1] = have_r ? static_cast<const char*>(a.r) + id * a.r_stride * (long long)sizeof(T) : nullptr;
+  // Two at a time are neighbours, so that a team has consecutive rows; single ones are dealt out one by one (8192 x 4096 fp32 91 us, 100 with
+  // consecutive rows).
+  const int step = kTwo ? 1 : p.total_teams, begin = kTwo ? id * p.rows_each + min(id, p.rows_over) : id;
+  const int end = kTwo ? begin + p.rows_each + (id < p.rows_over) : a.rows;
+  ring.step[0] = step * a.y_stride * (long long)sizeof(T);
+  ring.step[1] = step * a.r_stride * (long long)sizeof(T);
+  ring.from[0] = static_cast<const char*>(a.y) + begin * a.y_stride * (long long)sizeof(T);
+  ring.from[1] = have_r ? static_cast<const char*>(a.r) + begin * a.r_stride * (long long)sizeof(T) : nullptr;
   ring.at0 = own + team_ring_at(n, have_gate);
   ring.bars = smem_u32(own + kTeamBox);
   ring.parity = 0;
   ring.slots = p.slots, ring.row_bytes = p.row_bytes, ring.operands = p.operands, ring.slot = 0;
-  ring.left = id < a.rows ? (a.rows - 1 - id) / p.total_teams + 1 : 0;
+  ring.left = begin < end ? (end - 1 - begin) / step + 1 : 0;
   if (t == 0) ring.begin();
   row_ctl_begin(ctl);
   if (kN1) lay_vectors<4>(const_cast<float*>(vec), a, {a.w2, a.b2, a.w1, a.b1});
@@ -247,80 +257,131 @@ __global__ void __launch_bounds__(768, 1) souffle_residual_norm_rows(const NormA
   __syncthreads();
 
   auto has = [&](int i) { return kFull || cols.has(i, 0); };
-  auto norm = [&](F8 (&x)[kGroups], bool rms, float eps, const float* w, const float* b) {
-    float mean_w = 0.0f, m2 = 0.0f;
-    if (!rms) {
-      float sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kGroups; ++i) sum += sum8(x[i]);
-      mean_w = warp_total(sum) * team.inv_warp_cols;
-#pragma unroll
-      for (int i = 0; i < kGroups; ++i) x[i] = add8(x[i], has(i) ? -mean_w : 0.0f);
-    }
-#pragma unroll
-    for (int i = 0; i < kGroups; ++i) m2 += dot8(x[i], x[i]);
-    m2 = warp_total(m2);
-    if (team.warps > 1) {
-      float4 st[1];
-      team.merge<1>({mean_w}, {m2}, st);
-      m2 = st[0].y;
-      if (!rms) {
-#pragma unroll
-        for (int i = 0; i < kGroups; ++i) x[i] = add8(x[i], has(i) ? mean_w - st[0].x : 0.0f);
-      }
-    }
-    const float rstd = rsqrtf(m2 * team.inv_cols + eps);
+  const int per_gate = have_gate ? a.rows / a.gate_rows : 0x7fffffff;
+  int gate_at = 0, gate_end = have_gate ? 0 : 0x7fffffff;        // rows below gate_end have the gate that is in shared memory
+  auto lay_gate = [&] {                        // every thread brings the columns that it will read
 #pragma unroll
     for (int i = 0; i < kGroups; ++i)
-      if (has(i)) x[i] = fma8(mul8(x[i], rstd), read_plane(w + 256 * i), read_plane(b + 256 * i));
+      if (have_gate && has(i)) write_plane(gate_s + 256 * i, mul8(read_param(a, a.gate, (long long)gate_at * n + cols.at(i, 0)), a.beta));
   };
 
-  const int per_gate = have_gate ? a.rows / a.gate_rows : 0;
-  int gate_end = 0;                            // rows below it have the gate that is in shared memory
-  for (int row = id; row < a.rows; row += p.total_teams) {
-    if (have_gate && row >= gate_end) {        // every thread brings the columns that it will read
-      const int at = row / per_gate;
-      gate_end = (at + 1) * per_gate;
+  // kRows neighbouring rows that share a gate: what is read and decided for both is so once, and their chains of shuffles overlap
+  auto rows_of = [&](auto rows_c, int row) {
+    constexpr int kRows = decltype(rows_c)::value;
+    auto norm = [&](F8 (&x)[kRows][kGroups], bool rms, float eps, const float* w, const float* b) {
+      float mean_w[kRows], m2[kRows], rstd[kRows];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) mean_w[r] = 0.0f;
+      if (!rms) {
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          float sum = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kGroups; ++i) sum += sum8(x[r][i]);
+          mean_w[r] = warp_total(sum) * team.inv_warp_cols;
+        }
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+#pragma unroll
+          for (int i = 0; i < kGroups; ++i) x[r][i] = add8(x[r][i], has(i) ? -mean_w[r] : 0.0f);
+      }
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        m2[r] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i) m2[r] += dot8(x[r][i], x[r][i]);
+        m2[r] = warp_total(m2[r]);
+      }
+      if (team.warps > 1) {
+        float4 st[kRows];
+        team.merge(mean_w, m2, st);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          m2[r] = st[r].y;
+          if (!rms) {
+#pragma unroll
+            for (int i = 0; i < kGroups; ++i) x[r][i] = add8(x[r][i], has(i) ? mean_w[r] - st[r].x : 0.0f);
+          }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) rstd[r] = rsqrtf(m2[r] * team.inv_cols + eps);
 #pragma unroll
       for (int i = 0; i < kGroups; ++i)
-        if (has(i)) write_plane(gate_s + 256 * i, mul8(read_param(a, a.gate, (long long)at * n + cols.at(i, 0)), a.beta));
-    }
-    const T* slot = reinterpret_cast<const T*>(ring.wait(ctl.wait)) + cols.first;
-    F8 x[kGroups];
+        if (has(i)) {
+          const F8 wi = read_plane(w + 256 * i), bi = read_plane(b + 256 * i);
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i) x[i] = has(i) ? expand(read16(slot + 256 * i)) : all8(0.0f);
+          for (int r = 0; r < kRows; ++r) x[r][i] = fma8(mul8(x[r][i], rstd[r]), wi, bi);
+        }
+    };
+    const T* slot[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) slot[r] = reinterpret_cast<const T*>(ring.wait(ctl.wait, r)) + cols.first;
+    F8 x[kRows][kGroups];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) x[r][i] = has(i) ? expand(read16(slot[r] + 256 * i)) : all8(0.0f);
     if (kN1) norm(x, a.branch_norm == SOUFFLE_NORM_RMS, a.eps1, vec_s + 2 * plane, vec_s + 3 * plane);
     if (have_gate) {
 #pragma unroll
       for (int i = 0; i < kGroups; ++i)
-        if (has(i)) x[i] = mul8(x[i], read_plane(gate_s + 256 * i));
-    } else {
+        if (has(i)) {
+          const F8 gi = read_plane(gate_s + 256 * i);
 #pragma unroll
-      for (int i = 0; i < kGroups; ++i) x[i] = mul8(x[i], a.beta);
+          for (int r = 0; r < kRows; ++r) x[r][i] = mul8(x[r][i], gi);
+        }
+    } else if (a.beta != 1.0f) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i) x[r][i] = mul8(x[r][i], a.beta);
     }
     if (have_r) {
 #pragma unroll
-      for (int i = 0; i < kGroups; ++i)
-        if (has(i)) x[i] = fma8(expand(read16(slot + n + 256 * i)), a.alpha, x[i]);
+      for (int r = 0; r < kRows; ++r)
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i)
+          if (has(i)) x[r][i] = fma8(expand(read16(slot[r] + n + 256 * i)), a.alpha, x[r][i]);
     }
     if (team.warps == 1) __syncwarp();
     else team.meet();
-    ring.release(t == 0);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) ring.release(t == 0);
     if (a.s) {
       T* s = static_cast<T*>(a.s) + row * a.s_stride + cols.first;
 #pragma unroll
-      for (int i = 0; i < kGroups; ++i)
-        if (has(i)) write16(s + 256 * i, narrow<T>(x[i]));
+      for (int r = 0; r < kRows; ++r)
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i)
+          if (has(i)) write16(s + r * a.s_stride + 256 * i, narrow<T>(x[r][i]));
     }
-    if (a.out_norm == SOUFFLE_NORM_NONE) continue;
+    if (a.out_norm == SOUFFLE_NORM_NONE) return;
     norm(x, a.out_norm == SOUFFLE_NORM_RMS, a.eps2, vec_s, vec_s + plane);
     if (a.o) {
       T* o = static_cast<T*>(a.o) + row * a.o_stride + cols.first;
 #pragma unroll
-      for (int i = 0; i < kGroups; ++i)
-        if (has(i)) write16(o + 256 * i, narrow<T>(x[i]));
+      for (int r = 0; r < kRows; ++r)
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i)
+          if (has(i)) write16(o + r * a.o_stride + 256 * i, narrow<T>(x[r][i]));
     }
-    if (a.q) quantise_row<kGroups>(team, cols, x, a.q + row * a.q_stride, a.q_scale + row);
+    if (a.q) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) quantise_row<kGroups>(team, cols, x[r], a.q + (row + r) * a.q_stride, a.q_scale + row + r);
+    }
+  };
+
+  for (int row = begin; row < end;) {
+    if (row >= gate_end) {
+      gate_at = row / per_gate;
+      gate_end = (gate_at + 1) * per_gate;
+      lay_gate();
+    }
+    const bool two = kTwo && row + 1 < end && row + 1 < gate_end && p.slots >= kTwoSlots;
+    if (two) rows_of(std::integral_constant<int, kTwo ? 2 : 1>(), row);
+    else rows_of(std::integral_constant<int, 1>(), row);
+    row += two ? 2 : step;
   }
   row_ctl_end(ctl);
 }
@@ -519,8 +580,7 @@ __global__ void __launch_bounds__(kSharedSums ? 1024 : 32 * kGradWarps, 1) souff
 // overlap and which share what is read and decided for both; with two norms that takes 168 registers, so that a row has at most twelve
 // warps.  It is for a norm on the branch, where a row is three or four dependent exchanges (8192 x 768 fp16, both norms, 42.9 -> 34.2 us; 2048
 // bf16 107 -> 96); without one, one row at a time and sixteen warps are as fast or faster (16384 x 256 fp16 20.6 -> 19.5, 8192 x 2048
-// fp32 85 -> 74.6).  Two rows hold two slots, so that fewer than kTwoSlots leave none for the rows behind them.
-constexpr int kTwoSlots = 4;
+// fp32 85 -> 74.6).
 constexpr int grad_row_warps(bool both_norms, bool two) { return both_norms && two ? 12 : 16; }
 template <class T, bool kFull, bool kN1, bool kN2, bool kTwo>
 __global__ void __launch_bounds__(32 * grad_row_warps(kN1 && kN2, kTwo), 1) souffle_residual_norm_grad_rows(const NormGradArgs g, const RowPlan p) {
@@ -843,7 +903,7 @@ static NormArgs norm_args(const SouffleResidualNorm& d) {
   return a;
 }
 
-constexpr int kRowWarps = 24, kRowSmem = 220 * 1024;
+constexpr int kRowSmem = 220 * 1024;
 
 // How rows go through the ring: `groups` groups of eight columns a thread at most, operands of a row, vectors.  False: they do not fit.
 static bool row_plan(int rows, int cols, int elem, int operands, bool gate, int vectors, int max_groups, int max_warps, int sms, RowPlan* p, int* groups,
@@ -873,6 +933,8 @@ static bool row_plan(int rows, int cols, int elem, int operands, bool gate, int 
   const int need = (rows + p->teams - 1) / p->teams;
   *grid = need < sms ? need : sms;
   p->total_teams = *grid * p->teams;
+  p->rows_each = rows / p->total_teams;
+  p->rows_over = rows % p->total_teams;
   p->vectors = 64 + p->teams * p->team_bytes;
   *smem = p->vectors + vector_bytes;
   return true;
@@ -888,19 +950,25 @@ template <class F, class A> static int launch_rows(F fn, const A& a, const RowPl
   SF_CUDA(cudaGetLastError());
   return SOUFFLE_OK;
 }
-template <class T, bool kFull, int kGroups, bool kN1>
+template <class T, bool kFull, int kGroups, bool kN1, bool kTwo>
 static int forward_rows(const NormArgs& a, const RowPlan& p, int grid, int smem, int dev, cudaStream_t st) {
   static bool ready[kMaxDevices];
-  return launch_rows(souffle_residual_norm_rows<T, kFull, kGroups, kN1>, a, p, grid, smem, dev, ready, st);
+  return launch_rows(souffle_residual_norm_rows<T, kFull, kGroups, kN1, kTwo>, a, p, grid, smem, dev, ready, st);
 }
-template <class T, bool kFull, bool kN1>
+template <class T, bool kFull, bool kN1, bool kTwo>
 static int forward_rows(const NormArgs& a, const RowPlan& p, int groups, int grid, int smem, int dev, cudaStream_t st) {
   switch (groups) {
-    case 1: return forward_rows<T, kFull, 1, kN1>(a, p, grid, smem, dev, st);
-    case 2: return forward_rows<T, kFull, 2, kN1>(a, p, grid, smem, dev, st);
-    case 3: return forward_rows<T, kFull, 3, kN1>(a, p, grid, smem, dev, st);
-    default: return forward_rows<T, kFull, 4, kN1>(a, p, grid, smem, dev, st);
+    case 1: return forward_rows<T, kFull, 1, kN1, kTwo>(a, p, grid, smem, dev, st);
+    case 2: return forward_rows<T, kFull, 2, kN1, kTwo>(a, p, grid, smem, dev, st);
+    case 3: return forward_rows<T, kFull, 3, kN1, kTwo>(a, p, grid, smem, dev, st);
+    default: return forward_rows<T, kFull, 4, kN1, kTwo>(a, p, grid, smem, dev, st);
   }
+}
+template <class T, bool kN1>
+static int forward_rows(const NormArgs& a, const RowPlan& p, bool two, int groups, int grid, int smem, int dev, cudaStream_t st) {
+  const bool full = a.cols == 256 * p.warps * groups;
+  if (two) return full ? forward_rows<T, true, kN1, true>(a, p, groups, grid, smem, dev, st) : forward_rows<T, false, kN1, true>(a, p, groups, grid, smem, dev, st);
+  return full ? forward_rows<T, true, kN1, false>(a, p, groups, grid, smem, dev, st) : forward_rows<T, false, kN1, false>(a, p, groups, grid, smem, dev, st);
 }
 
 template <class T>
@@ -909,12 +977,10 @@ static int forward_launch(const NormArgs& a, bool vec, int sms, int dev, cudaStr
   int groups, grid, smem;
   const bool n1 = a.branch_norm != SOUFFLE_NORM_NONE;
   // Few rows: as many warps on a row as there are; many: as few as hold it
-  int max_groups = a.rows <= sms ? (a.cols + 256 * kRowWarps - 1) / (256 * kRowWarps) : 4;
-  if (vec && row_plan(a.rows, a.cols, sizeof(T), a.r ? 2 : 1, a.gate, n1 ? 4 : 2, max_groups, kRowWarps, sms, &p, &groups, &grid, &smem)) {
-    const bool full = a.cols == 256 * p.warps * groups;
-    if (n1) return full ? forward_rows<T, true, true>(a, p, groups, grid, smem, dev, st) : forward_rows<T, false, true>(a, p, groups, grid, smem, dev, st);
-    return full ? forward_rows<T, true, false>(a, p, groups, grid, smem, dev, st) : forward_rows<T, false, false>(a, p, groups, grid, smem, dev, st);
-  }
+  const bool few = a.rows <= sms, two = !few && a.cols <= 1024;
+  const int max_groups = few ? (a.cols + 256 * row_warps(false) - 1) / (256 * row_warps(false)) : 4;
+  if (vec && row_plan(a.rows, a.cols, sizeof(T), a.r ? 2 : 1, a.gate, n1 ? 4 : 2, max_groups, row_warps(two), sms, &p, &groups, &grid, &smem))
+    return n1 ? forward_rows<T, true>(a, p, two, groups, grid, smem, dev, st) : forward_rows<T, false>(a, p, two, groups, grid, smem, dev, st);
   const int warps = (a.cols + 255) / 256, threads = warps == 1 ? 128 : 32 * warps, teams = threads / (32 * warps);
   souffle_residual_norm_any<T><<<(a.rows + teams - 1) / teams, threads, 0, st>>>(a, warps);
   SF_CUDA(cudaGetLastError());

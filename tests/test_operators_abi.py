@@ -120,7 +120,7 @@ def test_the_operators_kernels_keep_their_values_in_registers():
     pairs = {k: v for k, v in usage.items() if "souffle_int8_pairs" in k}
     rows = {k: v for k, v in usage.items() if "souffle_residual_norm_rows" in k}
     grads = {k: v for k, v in usage.items() if "souffle_residual_norm_grad_rows" in k}
-    assert len(pairs) == 6 and len(rows) == 48 and len(grads) == 30
+    assert len(pairs) == 6 and len(rows) == 96 and len(grads) == 30
     for k, (regs, st, ld) in {**pairs, **rows, **grads}.items():
         limit = 0 if "pairs" in k else 64 if "norm_rows" in k else 128
         assert st <= limit and ld <= limit, f"{k} spills ({st} B stores, {ld} B loads, {regs} registers)"
