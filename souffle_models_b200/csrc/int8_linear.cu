@@ -146,7 +146,7 @@ __device__ __forceinline__ float activate(float v, int act) {
 
 // 16 bytes of a row from column k on, zeros past `inner`
 __device__ __forceinline__ int4 load16(const signed char* row, int k, int inner) {
-  if (k + 16 <= inner) return __ldg(reinterpret_cast<const int4*>(row + k));
+  if (k + 16 <= inner) return *reinterpret_cast<const int4*>(row + k);
   int w[4] = {0, 0, 0, 0};
   for (int i = 0; i < 16 && k + i < inner; ++i) w[i >> 2] |= (int)(uint32_t)(uint8_t)row[k + i] << (8 * (i & 3));
   return make_int4(w[0], w[1], w[2], w[3]);
@@ -215,7 +215,7 @@ template <int kTok> __device__ __forceinline__ void few_outputs(const LinearArgs
   }
 }
 
-// of rows that are quantised already
+// of quantised rows.  Behind the kernel that quantises them its blocks may be there before that has ended: they ask for weights and wait.
 template <int kTok>
 __global__ void __launch_bounds__(32 * kFewWarps) souffle_int8_few(const LinearArgs a) {
   __shared__ FewSmem sm;
@@ -224,6 +224,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) souffle_int8_few(const LinearA
   const signed char* x = static_cast<const signed char*>(a.x);
   int4 w[kAhead][2];
   few_weights(a, n0, g, t, warp, w);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (threadIdx.x < 8 * kTok) sm.scale[threadIdx.x] = m0 + (int)threadIdx.x < a.rows ? a.x_scale[m0 + threadIdx.x] : 0.0f;
   int acc[kTok][4] = {};
   few_product<kTok>(a, n0, warp, g, t, w, acc, [&](int j, int k) {
@@ -659,9 +660,10 @@ static int pairs_launch(const LinearArgs& a, bool behind_quantisation, int sms, 
 }
 
 // Up to kFewRows rows the legacy tensor path, which needs no tiles of 256 rows, is as fast or faster, as long as it does not read too many
-// weights (all of them for every sixteen rows): 64 x 768 x 3072 6.9 us against 7.3, but 48 x 4096 x 4096 20.2 against 10.7.
+// weights (all of them for every sixteen rows): 48 x 768 x 3072 4.5 us against 6.6, but 64 x 768 x 3072 6.9 and 48 x 4096 x 4096 20.2 against
+// 10.7.  Floating rows, the quantisation with them: 5.9 against 8.1, and 8.3 against 8.1.
 constexpr int kFewRows = 64;
-constexpr long long kFewWeights = 12 << 20;
+constexpr long long kFewWeights = 8 << 20;
 static bool few_rows(int rows, int inner, int cols) {
   return rows <= kFewRows && (rows <= 8 || (rows + 15) / 16 * (long long)inner * cols <= kFewWeights);
 }
@@ -750,8 +752,17 @@ int souffle_int8_linear_forward(const SouffleInt8Linear* call, souffle_stream_t 
     if (d.out_dtype == SOUFFLE_F32) return pairs_launch<float>(a, !given, sms, dev, st);
     return d.out_dtype == SOUFFLE_F16 ? pairs_launch<__half>(a, !given, sms, dev, st) : pairs_launch<__nv_bfloat16>(a, !given, sms, dev, st);
   }
-  souffle_int8_few<2><<<dim3((d.cols + 15) / 16, (d.rows + 15) / 16), 32 * kFewWarps, 0, st>>>(a);
-  SF_CUDA(cudaGetLastError());
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((d.cols + 15) / 16, (d.rows + 15) / 16);
+  cfg.blockDim = dim3(32 * kFewWarps);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = given ? 0 : 1;
+  SF_CUDA(cudaLaunchKernelEx(&cfg, souffle_int8_few<2>, a));
   return SOUFFLE_OK;
 }
 
