@@ -151,6 +151,7 @@ PyObject* int8_linear(PyObject* const* args) {
   const bool given = x.scalar_type() == at::kChar;
   d.x_dtype = given ? (int)SOUFFLE_I8 : code_of(x.scalar_type());
   if (!x.is_cuda() || d.x_dtype < 0) refuse("x must be an int8, float32, float16 or bfloat16 CUDA tensor");
+  if (x.requires_grad() && c10::GradMode::is_enabled()) refuse("a product in 8 bits has no gradient: x requires one");
   d.activation = (int)number(args[5]);
   d.out_dtype = (int)number(args[6]);
   if (d.out_dtype < 0) d.out_dtype = given ? (int)SOUFFLE_F16 : d.x_dtype;

@@ -46,7 +46,8 @@ def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: O
                 x_scale: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """x [..., K], int8 with `x_scale` [rows] (see quantize_rows) or floating (quantised on the way); w int8 [N, K] with rows a multiple
     of 16 bytes apart and w_scale [N] (see quantize_weight); bias [N] in the output's type; activation none, relu or gelu (tanh form).
-    Returns [..., N] in `out_dtype`, by default x's type, float16 for int8 rows.  K <= 131072.  Asynchronous."""
+    Returns [..., N] in `out_dtype`, by default x's type, float16 for int8 rows.  K <= 131072.  Asynchronous.
+    Has no gradient: where gradients are recorded, an x that requires one is refused."""
     act, out = _ACTIVATIONS.get(activation), -1 if out_dtype is None else _lib.DTYPE_CODES.get(out_dtype)
     if act is None or out is None:
         raise ValueError(f"out_dtype is float32, float16 or bfloat16 and activation {', '.join(_ACTIVATIONS)}: got {out_dtype}, {activation}")

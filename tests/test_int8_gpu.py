@@ -199,6 +199,17 @@ def test_refusals():
             i8.quantize_rows(bad)
 
 
+def test_an_input_that_requires_a_gradient_is_refused():
+    i8 = _int8()
+    w, sw = _rows8(8, 64)
+    x = torch.ones(4, 64, device="cuda", requires_grad=True)
+    with pytest.raises(ValueError):
+        i8.int8_linear(x, w, sw)
+    with torch.no_grad():
+        got = i8.int8_linear(x, w, sw)
+    assert torch.equal(got, i8.int8_linear(x.detach(), w, sw)) and not got.requires_grad
+
+
 @pytest.mark.parametrize("rows", [5, 200])
 def test_on_another_stream_and_in_a_graph(rows):
     i8 = _int8()
