@@ -162,38 +162,37 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], int a0, int a1, int a2, int 
 // the columns inside the 64 does not matter to the sum.  What bounds it is the latency of memory: a warp asks for the weights of
 // kAhead chunks at once, the first ones before anything else.
 constexpr int kFewWarps = 8, kAhead = 4;
-struct FewSmem {
-  int part[kFewWarps][2][16 * 8];
+template <int kWarps> struct FewSmem {
+  int part[kWarps][2][16 * 8];
   float scale[16];
-  alignas(16) char box[kFewWarps][kTeamBox];
 };
-__device__ __forceinline__ void few_weights(const LinearArgs& a, int n0, int g, int t, int chunk, int4 (&w)[kAhead][2]) {
+template <int kWarps> __device__ __forceinline__ void few_weights(const LinearArgs& a, int n0, int g, int t, int chunk, int4 (&w)[kAhead][2]) {
   const int4 none = make_int4(0, 0, 0, 0);
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) {
-    const int k = 64 * (chunk + i * kFewWarps) + 16 * t;
+    const int k = 64 * (chunk + i * kWarps) + 16 * t;
     w[i][0] = k < a.inner && n0 + g < a.cols ? load16(a.w + (n0 + g) * a.w_stride, k, a.inner) : none;
     w[i][1] = k < a.inner && n0 + g + 8 < a.cols ? load16(a.w + (n0 + g + 8) * a.w_stride, k, a.inner) : none;
   }
 }
-template <int kTok, class F> __device__ __forceinline__ void few_product(const LinearArgs& a, int n0, int warp, int g, int t, int4 (&w)[kAhead][2], int (&acc)[kTok][4], F token) {
+template <int kTok, int kWarps, class F> __device__ __forceinline__ void few_product(const LinearArgs& a, int n0, int warp, int g, int t, int4 (&w)[kAhead][2], int (&acc)[kTok][4], F token) {
   const int chunks = (a.inner + 63) / 64;
-  for (int chunk = warp; chunk < chunks; chunk += kAhead * kFewWarps) {
+  for (int chunk = warp; chunk < chunks; chunk += kAhead * kWarps) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      if (chunk + i * kFewWarps >= chunks) break;
+      if (chunk + i * kWarps >= chunks) break;
 #pragma unroll
       for (int j = 0; j < kTok; ++j) {
-        const int4 b = token(j, 64 * (chunk + i * kFewWarps) + 16 * t);
+        const int4 b = token(j, 64 * (chunk + i * kWarps) + 16 * t);
         mma_s8(acc[j], w[i][0].x, w[i][1].x, w[i][0].y, w[i][1].y, b.x, b.y);
         mma_s8(acc[j], w[i][0].z, w[i][1].z, w[i][0].w, w[i][1].w, b.z, b.w);
       }
     }
-    if (chunk + kAhead * kFewWarps < chunks) few_weights(a, n0, g, t, chunk + kAhead * kFewWarps, w);
+    if (chunk + kAhead * kWarps < chunks) few_weights<kWarps>(a, n0, g, t, chunk + kAhead * kWarps, w);
   }
 }
 // The warps' sums become outputs; `scale` has the tokens' scales.
-template <int kTok> __device__ __forceinline__ void few_outputs(const LinearArgs& a, FewSmem& sm, int n0, int m0, int warp, int g, int t, const int (&acc)[kTok][4], const float* scale) {
+template <int kTok, int kWarps> __device__ __forceinline__ void few_outputs(const LinearArgs& a, FewSmem<kWarps>& sm, int n0, int m0, int warp, int g, int t, const int (&acc)[kTok][4], const float* scale) {
 #pragma unroll
   for (int i = 0; i < kTok; ++i) {       // [token][channel]
     int* p = sm.part[warp][i];
@@ -203,12 +202,12 @@ template <int kTok> __device__ __forceinline__ void few_outputs(const LinearArgs
     p[(2 * t + 1) * 16 + g + 8] = acc[i][3];
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < 128 * kTok; e += 32 * kFewWarps) {
+  for (int e = threadIdx.x; e < 128 * kTok; e += 32 * kWarps) {
     const int token = e >> 4, m = m0 + token, n = n0 + (e & 15);
     if (m >= a.rows || n >= a.cols) continue;
     int sum = 0;
 #pragma unroll
-    for (int w = 0; w < kFewWarps; ++w) sum += sm.part[w][e >> 7][e & 127];
+    for (int w = 0; w < kWarps; ++w) sum += sm.part[w][e >> 7][e & 127];
     float v = (float)sum * scale[token] * a.w_scale[n];
     if (a.bias) v += load_value(a.bias, a.out_dtype, n);
     store_value(a.out, a.out_dtype, m * a.out_stride + n, activate(v, a.act));
@@ -218,41 +217,42 @@ template <int kTok> __device__ __forceinline__ void few_outputs(const LinearArgs
 // of quantised rows.  Behind the kernel that quantises them its blocks may be there before that has ended: they ask for weights and wait.
 template <int kTok>
 __global__ void __launch_bounds__(32 * kFewWarps) souffle_int8_few(const LinearArgs a) {
-  __shared__ FewSmem sm;
+  __shared__ FewSmem<kFewWarps> sm;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 8 * kTok;
   const signed char* x = static_cast<const signed char*>(a.x);
   int4 w[kAhead][2];
-  few_weights(a, n0, g, t, warp, w);
+  few_weights<kFewWarps>(a, n0, g, t, warp, w);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (threadIdx.x < 8 * kTok) sm.scale[threadIdx.x] = m0 + (int)threadIdx.x < a.rows ? a.x_scale[m0 + threadIdx.x] : 0.0f;
   int acc[kTok][4] = {};
-  few_product<kTok>(a, n0, warp, g, t, w, acc, [&](int j, int k) {
+  few_product<kTok, kFewWarps>(a, n0, warp, g, t, w, acc, [&](int j, int k) {
     const int m = m0 + 8 * j + g;
     return m < a.rows && k < a.inner ? load16(x + m * a.x_stride, k, a.inner) : make_int4(0, 0, 0, 0);
   });
-  few_outputs<kTok>(a, sm, n0, m0, warp, g, t, acc, sm.scale);
+  few_outputs<kTok, kFewWarps>(a, sm, n0, m0, warp, g, t, acc, sm.scale);
 }
 
-// of floating rows, at most 8 kTok: each CTA quantises them for itself, into shared memory, a token by 8 / tokens warps (one launch, and no
+// of floating rows, at most 8 kTok: each CTA quantises them for itself, into shared memory, a token by kWarps / tokens warps (one launch, and no
 // rows or scales through memory).  kVec as in Columns.
 constexpr int kFewCached = 4, kFewFloatRows = 16, kFewFloatBytes = 96 * 1024;
 __host__ __device__ inline int few_pitch(int inner) {          // bytes of a token: zeros to a multiple of 64, an odd one, so that eight tokens' 64 bytes lie in all banks
   const int n = (inner + 63) / 64;
   return 64 * (n | 1);
 }
-template <class T, bool kVec, int kTok>
-__global__ void __launch_bounds__(32 * kFewWarps) souffle_int8_few_floats(const LinearArgs a, int warps_per_token) {
+template <class T, bool kVec, int kTok, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps) souffle_int8_few_floats(const LinearArgs a, int warps_per_token) {
   extern __shared__ __align__(16) signed char tokens[];
-  __shared__ FewSmem sm;
+  __shared__ FewSmem<kWarps> sm;
+  __shared__ __align__(16) char box[kFewWarps][kTeamBox];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, n0 = blockIdx.x * 16;
   int4 w[kAhead][2];
-  few_weights(a, n0, g, t, warp, w);
-  const int pitch = few_pitch(a.inner), teams = kFewWarps / warps_per_token, mine = warp / warps_per_token;
+  few_weights<kWarps>(a, n0, g, t, warp, w);
+  const int pitch = few_pitch(a.inner), teams = kWarps / warps_per_token, mine = warp / warps_per_token;
   const Columns<kVec> cols = {(int)threadIdx.x - mine * 32 * warps_per_token, 32 * warps_per_token, a.inner};
   Team team;
-  team.begin(sm.box[mine], warps_per_token, warp - mine * warps_per_token, 1 + mine, cols, 0);
-  for (int i = a.inner + threadIdx.x; i < pitch; i += 32 * kFewWarps)
+  team.begin(box[mine % kFewWarps], warps_per_token, warp - mine * warps_per_token, 1 + mine, cols, 0);
+  for (int i = a.inner + threadIdx.x; i < pitch; i += 32 * kWarps)
     for (int m = 0; m < a.rows; ++m) tokens[m * pitch + i] = 0;
   if (warps_per_token > 1) team.meet();
   const int groups = (a.inner + 256 * warps_per_token - 1) / (256 * warps_per_token);
@@ -285,11 +285,11 @@ __global__ void __launch_bounds__(32 * kFewWarps) souffle_int8_few_floats(const 
   }
   __syncthreads();
   int acc[kTok][4] = {};
-  few_product<kTok>(a, n0, warp, g, t, w, acc, [&](int j, int k) {
+  few_product<kTok, kWarps>(a, n0, warp, g, t, w, acc, [&](int j, int k) {
     const int m = 8 * j + g;
     return m < a.rows ? *reinterpret_cast<const int4*>(tokens + m * pitch + k) : make_int4(0, 0, 0, 0);
   });
-  few_outputs<kTok>(a, sm, n0, 0, warp, g, t, acc, sm.scale);
+  few_outputs<kTok, kWarps>(a, sm, n0, 0, warp, g, t, acc, sm.scale);
 }
 
 // ---- many tokens -------------------------------------------------------------------------------------------------
@@ -673,20 +673,27 @@ constexpr long long kFewFloatReads = 6 << 20;
 static bool few_floats(int rows, int inner, int cols) {
   return rows <= kFewFloatRows && (long long)rows * few_pitch(inner) <= kFewFloatBytes && (long long)rows * inner * ((cols + 15) / 16) <= kFewFloatReads;
 }
-template <class T>
+template <class T, int kWarps>
 static int few_launch(const LinearArgs& a, int dev, cudaStream_t st) {
   const bool vec = a.inner % 8 == 0 && ((uintptr_t)a.x & 15u) == 0 && (a.x_stride * (long long)sizeof(T)) % 16 == 0;
-  const int warps = a.rows == 1 ? 8 : a.rows == 2 ? 4 : a.rows <= 4 ? 2 : 1, smem = a.rows * few_pitch(a.inner);
-  auto fn = a.rows <= 8 ? (vec ? souffle_int8_few_floats<T, true, 1> : souffle_int8_few_floats<T, false, 1>)
-                        : (vec ? souffle_int8_few_floats<T, true, 2> : souffle_int8_few_floats<T, false, 2>);
+  const int tokens = a.rows == 1 ? 1 : a.rows == 2 ? 2 : a.rows <= 4 ? 4 : 8, warps = a.rows <= 8 ? kWarps / tokens : 1, smem = a.rows * few_pitch(a.inner);
+  auto fn = a.rows <= 8 ? (vec ? souffle_int8_few_floats<T, true, 1, kWarps> : souffle_int8_few_floats<T, false, 1, kWarps>)
+                        : (vec ? souffle_int8_few_floats<T, true, 2, kWarps> : souffle_int8_few_floats<T, false, 2, kWarps>);
   static bool ready[2][2][kMaxDevices];
   if (!ready[a.rows <= 8][vec][dev]) {
     SF_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewFloatBytes));
     ready[a.rows <= 8][vec][dev] = true;
   }
-  fn<<<(a.cols + 15) / 16, 32 * kFewWarps, smem, st>>>(a, warps);
+  fn<<<(a.cols + 15) / 16, 32 * kWarps, smem, st>>>(a, warps);
   SF_CUDA(cudaGetLastError());
   return SOUFFLE_OK;
+}
+// Sixteen warps where each SM has one CTA at most and eight would come back for more weights or have two tokens each: 7 x 3072 x 768 6.4 us
+// with eight, 5.2 with sixteen, 16 x 768 x 768 4.5 and 4.15; but 8 x 768 x 768 3.65 and 3.9, and 8 x 768 x 3072, of 192 CTAs, 4.0 and 6.4.
+template <class T>
+static int few_launch(const LinearArgs& a, int sms, int dev, cudaStream_t st) {
+  const bool more = (a.cols + 15) / 16 <= sms && (a.rows > 8 || a.inner > 64 * kAhead * kFewWarps);
+  return more ? few_launch<T, 2 * kFewWarps>(a, dev, st) : few_launch<T, kFewWarps>(a, dev, st);
 }
 
 }  // namespace souffle
@@ -739,8 +746,8 @@ int souffle_int8_linear_forward(const SouffleInt8Linear* call, souffle_stream_t 
   a.x_stride = d.x_stride; a.w_stride = d.w_stride; a.out_stride = d.out_stride;
   a.x = d.x; a.x_scale = d.x_scale; a.w = static_cast<const signed char*>(d.w); a.w_scale = d.w_scale; a.bias = d.bias; a.out = d.out;
   if (!given && few_floats(d.rows, d.inner, d.cols)) {
-    if (d.x_dtype == SOUFFLE_F32) return few_launch<float>(a, dev, st);
-    return d.x_dtype == SOUFFLE_F16 ? few_launch<__half>(a, dev, st) : few_launch<__nv_bfloat16>(a, dev, st);
+    if (d.x_dtype == SOUFFLE_F32) return few_launch<float>(a, sms, dev, st);
+    return d.x_dtype == SOUFFLE_F16 ? few_launch<__half>(a, sms, dev, st) : few_launch<__nv_bfloat16>(a, sms, dev, st);
   }
   if (!given) {
     float* scale = static_cast<float*>(d.workspace);

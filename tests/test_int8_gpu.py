@@ -115,6 +115,12 @@ def test_products_of_floating_rows(rows, inner, cols, dtype):
     _check(*_quantise(x), w, sw, torch.randn(cols, device="cuda").to(dtype), "gelu", dtype, x=x)
 
 
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 8, 9, 16])
+@pytest.mark.parametrize("inner,cols", [(2048, 40), (2049, 17), (2056, 2368), (2056, 2369), (5000, 33)])
+def test_products_of_few_rows_and_long_ones(rows, inner, cols):
+    test_products_of_floating_rows(rows, inner, cols, FLOATS[(rows + inner) % 3])
+
+
 @pytest.mark.parametrize("rows,inner,cols", [(1, 131072, 3), (20, 131072, 17), (140, 131072, 130), (300, 131072, 300)])
 def test_sums_reach_the_end_of_32_bits(rows, inner, cols):
     q, w = _int8().empty_rows(rows, inner, "cuda")[0].fill_(127), _int8().empty_rows(cols, inner, "cuda")[0].fill_(127)
